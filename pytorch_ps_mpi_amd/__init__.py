@@ -10,7 +10,7 @@ compute.
 
 Public API (reference parity: __init__.py:1 exported MPI_PS, Adam, SGD):
 
-    from pytorch_ps_mpi_amd import PS, SGD, Adam
+    from pytorch_ps_mpi_amd import PS, SGD, Adam, AdamW
     opt = SGD(model.named_parameters(), lr=0.1, momentum=0.9,
               code="topk:0.01", mode="async")
     loss.backward(); loss, metrics = opt.step(loss=loss)
@@ -19,19 +19,19 @@ Public API (reference parity: __init__.py:1 exported MPI_PS, Adam, SGD):
 from . import codecs, models, ops
 from .codecs import (HostCodec, Identity, QuantInt8, TopK,
                      TopKThreshold, get_codec)
-from .optim import PS, SGD, Adam
+from .optim import PS, SGD, Adam, AdamW
 from .parallel.comm import Comm, init_distributed
 
 def MPI_PS(named_params, *, optim="sgd", code=None, **kwargs):
     """Reference-compatible constructor (ps.py:53-59): selects the update
-    rule via ``optim='sgd'|'adam'`` and takes the codec as ``code``."""
-    cls = {"sgd": SGD, "adam": Adam}.get(optim)
+    rule via ``optim='sgd'|'adam'|'adamw'`` and takes the codec as ``code``."""
+    cls = {"sgd": SGD, "adam": Adam, "adamw": AdamW}.get(optim)
     if cls is None:
-        raise ValueError(f"optim must be 'sgd' or 'adam', got {optim!r}")
+        raise ValueError(f"optim must be 'sgd', 'adam' or 'adamw', got {optim!r}")
     return cls(named_params, code=code, **kwargs)
 
 __all__ = [
-    "PS", "MPI_PS", "SGD", "Adam",
+    "PS", "MPI_PS", "SGD", "Adam", "AdamW",
     "Identity", "TopK", "TopKThreshold", "QuantInt8", "HostCodec",
     "get_codec",
     "Comm", "init_distributed",

@@ -14,6 +14,8 @@ compression plugin (ps.py:18).
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 _EXT = None
@@ -88,6 +90,195 @@ def fused_adam(p, m1, m2, vmax, g, p_out, *, lr, beta1=0.9, beta2=0.999,
     p.addcdiv_(m1, denom, value=-(lr / bc1))
     if p_out is not None:
         p_out.copy_(p)
+
+
+# ---------------------------------------------------------------------------
+# AdamW over a packed set of tensors, states in 32 or 8 bits
+# ---------------------------------------------------------------------------
+
+ACHUNK = 256  # elements that share one decay factor and one 8-bit maximum
+_MASK32 = 0xffffffff
+
+
+def _chunks(n: int) -> int:
+    return (n + ACHUNK - 1) // ACHUNK
+
+
+class State8:
+    """A flat optimizer state in 8 bits: one code an element, one fp32 maximum
+    for each 256 elements.
+
+    Code k in 1..top stands for ``max * 2**((k - top) / 8)``, 0 for zero.
+    ``signed=True`` (first moment): bit 7 is the sign, top is 127.
+    ``signed=False`` (second moment, never negative): top is 255.
+    """
+
+    def __init__(self, codes, scales, signed):
+        if codes.dtype != torch.uint8 or codes.dim() != 1:
+            raise ValueError("State8 codes must be a flat uint8 tensor")
+        if scales.dtype != torch.float32 or scales.dim() != 1:
+            raise ValueError("State8 scales must be a flat float32 tensor")
+        if scales.numel() != _chunks(codes.numel()):
+            raise ValueError(
+                f"State8 of {codes.numel()} elements needs "
+                f"{_chunks(codes.numel())} scales, got {scales.numel()}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("State8 tensors must be contiguous")
+        if codes.device != scales.device:
+            raise ValueError("State8 tensors must be on one device")
+        self.codes, self.scales, self.signed = codes, scales, bool(signed)
+
+    @classmethod
+    def zeros(cls, n, signed, device=None):
+        return cls(torch.zeros(n, dtype=torch.uint8, device=device),
+                   torch.zeros(_chunks(n), device=device), signed)
+
+    def span(self, start, end):
+        """State8 of elements [start, end), sharing storage."""
+        if start % ACHUNK:
+            raise ValueError(f"a span starts at a multiple of {ACHUNK}")
+        if end % ACHUNK and end != self.codes.numel():
+            raise ValueError(f"a span ends at a multiple of {ACHUNK} or at "
+                             "the state's end")
+        return State8(self.codes[start:end],
+                      self.scales[start // ACHUNK:_chunks(end)], self.signed)
+
+    def values(self, dtype=torch.float32):
+        """What the codes stand for, as a new flat tensor."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("State8 values come as float32 or bfloat16")
+        n = self.codes.numel()
+        if _require_ext(self.codes):
+            out = torch.empty(n, dtype=dtype, device=self.codes.device)
+            _EXT.state8_values(self.codes, self.scales, out, self.signed)
+            return out
+        top = 127 if self.signed else 255
+        c = self.codes.int()
+        k = c & top
+        x = torch.exp2((k - top).float() / 8)
+        x = torch.where(k == 0, torch.zeros_like(x), x)
+        x = x * self.scales.repeat_interleave(ACHUNK)[:n]
+        return torch.where(c > top, -x, x).to(dtype)
+
+
+def _mix32(h):
+    h = h ^ (h >> 16)
+    h = (h * 0x7feb352d) & _MASK32
+    h = h ^ (h >> 15)
+    h = (h * 0x846ca68b) & _MASK32
+    return h ^ (h >> 16)
+
+
+def _state8_store(st, x, r16):
+    """Encode x (fp32) into st; r16 holds 16 random bits an element."""
+    n, nc = x.numel(), st.scales.numel()
+    top = 127 if st.signed else 255
+    pad = torch.zeros(nc * ACHUNK, dtype=torch.float32, device=x.device)
+    pad[:n] = x
+    a = pad.view(nc, ACHUNK).abs()
+    s = a.amax(1)
+    s = torch.where(torch.isfinite(s), s, torch.full_like(s, float("nan")))
+    e = top + 8 * torch.log2(
+        a / torch.where(s > 0, s, torch.ones_like(s))[:, None])
+    lo = e.floor()
+    u = torch.zeros(nc * ACHUNK, dtype=torch.float32, device=x.device)
+    u[:n] = (r16.float() + 0.5) / 65536
+    u = u.view(nc, ACHUNK)
+    up = torch.expm1((e - lo) * (math.log(2.0) / 8)) / (2 ** 0.125 - 1)
+    k = (lo + (u < up)).clamp(max=top)
+    if st.signed:
+        low = (u < torch.exp2((e - 1) / 8)).float()
+    else:
+        low = torch.ones_like(e)
+    k = torch.where(e < 1, low, k)
+    k = torch.where(a > 0, k, torch.zeros_like(k)).nan_to_num(0.0)
+    if st.signed:
+        k = k + 128 * ((pad.view(nc, ACHUNK) < 0) & (k > 0))
+    st.codes.copy_(k.to(torch.uint8).view(-1)[:n])
+    st.scales.copy_(s)
+
+
+def fused_adamw(p, m1, m2, g, p_out=None, *, lr, beta1=0.9, beta2=0.999,
+                eps=1e-8, wd=0.01, step=1, gscale=1.0, decay=None, offset=0,
+                seed=0):
+    """One AdamW step (decoupled decay, torch.optim.AdamW's formula) in place
+    over a packed set of tensors.
+
+    p, g : flat fp32.  p_out : optional bf16/fp32 model copy.
+    m1, m2 : both flat fp32, or both State8 (signed / unsigned).
+    decay : optional fp32 factor on ``wd`` for each 256 elements (tensors that
+        start at multiples of 256 get their own; None decays everything).
+    offset, seed : with 8-bit states a value between two codes is rounded up
+        with the probability that keeps its mean, from bits that depend on
+        (offset + element index, seed, step) alone: a buffer updated in parts
+        (``offset`` = where the part starts) rounds as it would in one.
+        An infinity or NaN makes the values of its 256 elements read as NaN.
+    """
+    n = p.numel()
+    eight = isinstance(m1, State8)
+    if eight != isinstance(m2, State8):
+        raise ValueError("m1 and m2 must both be fp32 or both State8")
+    if eight and not (m1.signed and not m2.signed):
+        raise ValueError("m1 is a signed State8, m2 an unsigned one")
+    step, offset = int(step), int(offset)
+    if step < 1:
+        raise ValueError("step counts from 1")
+    if offset < 0 or (eight and offset % ACHUNK):
+        raise ValueError(f"offset must be a multiple of {ACHUNK}, 0 or more")
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError("betas must be in [0, 1)")
+    flat = [("p", p), ("g", g)]
+    flat += [] if eight else [("m1", m1), ("m2", m2)]
+    for name, t in flat:
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32")
+        if t.numel() != n:
+            raise ValueError(f"{name} has {t.numel()} elements, p has {n}")
+    if eight and not (m1.codes.numel() == m2.codes.numel() == n):
+        raise ValueError("state and parameter lengths differ")
+    if decay is not None and (decay.dtype != torch.float32
+                              or not decay.is_contiguous()
+                              or decay.numel() != _chunks(n)):
+        raise ValueError(f"decay must be {_chunks(n)} contiguous float32 "
+                         "factors, one for each 256 elements")
+    if p_out is not None and (p_out.dtype not in (torch.float32,
+                                                  torch.bfloat16)
+                              or p_out.numel() != n
+                              or not p_out.is_contiguous()):
+        raise ValueError("p_out must be contiguous bf16/fp32 of p's length")
+    every = [t for _, t in flat[1:]] + [t for t in (p_out, decay)
+                                        if t is not None]
+    every += [m1.codes, m2.codes] if eight else []
+    if any(t.device != p.device for t in every):
+        raise ValueError("all tensors of fused_adamw must be on one device")
+    key = (int(seed) + 0x9e3779b9 * step) & _MASK32
+    bc1, bc2 = 1.0 - beta1 ** step, 1.0 - beta2 ** step
+    if _require_ext(p):
+        _EXT.fused_adamw(p, p_out, g, m1.codes if eight else m1,
+                         m2.codes if eight else m2,
+                         m1.scales if eight else None,
+                         m2.scales if eight else None, decay, offset,
+                         lr / bc1, lr * wd, beta1, beta2, bc2 ** -0.5, eps,
+                         gscale, key)
+        return
+    d = g * gscale
+    m = beta1 * (m1.values() if eight else m1) + (1.0 - beta1) * d
+    v = beta2 * (m2.values() if eight else m2) + (1.0 - beta2) * d * d
+    if decay is None:
+        p.mul_(1.0 - lr * wd)
+    else:
+        p.sub_(p * (lr * wd * decay).repeat_interleave(ACHUNK)[:n])
+    p.addcdiv_(m, (v.sqrt() * bc2 ** -0.5).add_(eps), value=-(lr / bc1))
+    if p_out is not None:
+        p_out.copy_(p)
+    if eight:
+        i = torch.arange(offset, offset + n, device=p.device)
+        r = _mix32((i & _MASK32) ^ _mix32((key + (i >> 32)) & _MASK32))
+        _state8_store(m1, m, r & 0xffff)
+        _state8_store(m2, v, r >> 16)
+    else:
+        m1.copy_(m)
+        m2.copy_(v)
 
 
 # ---------------------------------------------------------------------------

@@ -2,6 +2,7 @@
 // Pure HIP-side code (no CUDA compat paths): streams come from c10::hip.
 
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdint>
@@ -15,6 +16,13 @@ int ps_fused_adam(void* stream, float* p, float* m1, float* m2, float* vmax,
                   const float* g, void* p_out, int p_out_is_bf16, int64_t n,
                   float lr, float beta1, float beta2, float eps, float wd,
                   float bc1, float bc2_sqrt, int amsgrad, float gscale);
+int ps_fused_adamw(void* stream, float* p, void* out, int out_kind,
+                   const float* g, void* m, void* v, float* ms, float* vs,
+                   const float* decay, int64_t n, int64_t offset,
+                   float step_size, float lr_wd, double beta1, double beta2,
+                   float inv_bc2_sqrt, float eps, float gscale, uint32_t key);
+int ps_state8_values(void* stream, const uint8_t* codes, const float* scales,
+                     void* out, int out_is_bf16, int is_signed, int64_t n);
 int ps_reduce_accum(void* stream, float* dst, const void** srcs, int nsrc,
                     int src_is_bf16, int64_t n, float scale, float beta);
 int ps_f32_to_bf16(void* stream, const float* src, void* dst, int64_t n);
@@ -176,6 +184,86 @@ void fused_adam(at::Tensor p, at::Tensor m1, at::Tensor m2,
                          (float)beta2, (float)eps, (float)wd, (float)bc1,
                          (float)bc2_sqrt, amsgrad ? 1 : 0, (float)gscale),
            "fused_adam");
+}
+
+void check_same_device(const at::Tensor& a, const at::Tensor& t,
+                       const char* name) {
+  TORCH_CHECK(t.device() == a.device(), name, " is on another device");
+}
+
+void fused_adamw(at::Tensor p, c10::optional<at::Tensor> p_out, at::Tensor g,
+                 at::Tensor m, at::Tensor v, c10::optional<at::Tensor> ms,
+                 c10::optional<at::Tensor> vs,
+                 c10::optional<at::Tensor> decay, int64_t offset,
+                 double step_size, double lr_wd, double beta1, double beta2,
+                 double inv_bc2_sqrt, double eps, double gscale,
+                 int64_t key) {
+  const bool s8 = ms.has_value();
+  const int64_t n = p.numel(), chunks = (n + 255) / 256;
+  const auto st = s8 ? at::kByte : at::kFloat;
+  check_flat(p, at::kFloat, "param");
+  check_flat(g, at::kFloat, "grad");
+  check_flat(m, st, "exp_avg");
+  check_flat(v, st, "exp_avg_sq");
+  TORCH_CHECK(g.numel() == n && m.numel() == n && v.numel() == n,
+              "param/grad/state length mismatch");
+  TORCH_CHECK(s8 == vs.has_value(), "8-bit states need both scales");
+  for (const auto& t : {g, m, v}) check_same_device(p, t, "grad/state");
+  float *msp = nullptr, *vsp = nullptr;
+  if (s8) {
+    check_flat(*ms, at::kFloat, "exp_avg scales");
+    check_flat(*vs, at::kFloat, "exp_avg_sq scales");
+    TORCH_CHECK(ms->numel() == chunks && vs->numel() == chunks,
+                "one scale for each 256 elements");
+    check_same_device(p, *ms, "scales");
+    check_same_device(p, *vs, "scales");
+    msp = ms->data_ptr<float>();
+    vsp = vs->data_ptr<float>();
+  }
+  const float* dp = nullptr;
+  if (decay.has_value()) {
+    check_flat(*decay, at::kFloat, "decay");
+    check_same_device(p, *decay, "decay");
+    TORCH_CHECK(decay->numel() == chunks, "one decay for each 256 elements");
+    dp = decay->data_ptr<float>();
+  }
+  void* out_ptr = nullptr;
+  int kind = 0;
+  if (p_out.has_value()) {
+    check_flat(*p_out, p_out->scalar_type(), "p_out");
+    check_same_device(p, *p_out, "p_out");
+    TORCH_CHECK(p_out->numel() == n, "p_out length mismatch");
+    TORCH_CHECK(is_bf16(*p_out) || p_out->scalar_type() == at::kFloat,
+                "p_out dtype");
+    out_ptr = p_out->data_ptr();
+    kind = is_bf16(*p_out) ? 1 : 2;
+  }
+  const c10::DeviceGuard guard(p.device());
+  throw_on(ps_fused_adamw(cur_stream(p), p.data_ptr<float>(), out_ptr, kind,
+                          g.data_ptr<float>(), m.data_ptr(), v.data_ptr(), msp,
+                          vsp, dp, n, offset, (float)step_size, (float)lr_wd,
+                          beta1, beta2, (float)inv_bc2_sqrt,
+                          (float)eps, (float)gscale, (uint32_t)key),
+           "fused_adamw");
+}
+
+void state8_values(at::Tensor codes, at::Tensor scales, at::Tensor out,
+                   bool is_signed) {
+  check_flat(codes, at::kByte, "codes");
+  check_flat(scales, at::kFloat, "scales");
+  check_flat(out, out.scalar_type(), "out");
+  check_same_device(codes, scales, "scales");
+  check_same_device(codes, out, "out");
+  const int64_t n = codes.numel();
+  TORCH_CHECK(scales.numel() == (n + 255) / 256, "one scale per 256 elements");
+  TORCH_CHECK(out.numel() == n &&
+                  (is_bf16(out) || out.scalar_type() == at::kFloat),
+              "out must be bf16/f32 of the codes' length");
+  const c10::DeviceGuard guard(codes.device());
+  throw_on(ps_state8_values(cur_stream(codes), codes.data_ptr<uint8_t>(),
+                            scales.data_ptr<float>(), out.data_ptr(),
+                            is_bf16(out), is_signed ? 1 : 0, n),
+           "state8_values");
 }
 
 void reduce_accum(at::Tensor dst, std::vector<at::Tensor> srcs, double scale,
@@ -612,6 +700,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bn_bwd_dx", &bn_bwd_dx);
   m.def("fused_sgd", &fused_sgd, "fused SGD over flat fp32 buffers");
   m.def("fused_adam", &fused_adam, "fused Adam over flat fp32 buffers");
+  m.def("fused_adamw", &fused_adamw,
+        "AdamW over packed fp32 buffers, states in 32 or 8 bits");
+  m.def("state8_values", &state8_values, "values that 8-bit codes stand for");
   m.def("reduce_accum", &reduce_accum, "dst = beta*dst + scale*sum(srcs)");
   m.def("f32_to_bf16", &f32_to_bf16, "flat cast");
   m.def("bf16_to_f32", &bf16_to_f32, "flat cast");

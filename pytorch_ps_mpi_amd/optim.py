@@ -286,3 +286,83 @@ class Adam(PS):
         if self._vmax is not None:
             d["max_exp_avg_sq"] = self._vmax
         return d
+
+
+class AdamW(PS):
+    """AdamW (decoupled weight decay, torch.optim.AdamW's formula), fused
+    on-device over the flat space: one launch a bucket for all its tensors.
+
+    state_bits : 32, or 8 for states of one byte an element plus one fp32
+        maximum per 256 (ops.State8; rounded without bias, the same bits on
+        every rank and for every bucket size).
+    no_decay : optional ``f(name, param) -> bool``; parameters for which it is
+        true are not decayed (e.g. ``lambda n, p: p.dim() < 2``).
+    seed : chooses the rounding bits of 8-bit states.
+    """
+
+    def __init__(self, named_params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+                 weight_decay=0.01, state_bits=32, no_decay=None, seed=0,
+                 **ps_kwargs):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self.state_bits = int(state_bits)
+        self.seed = int(seed)
+        self._no_decay = no_decay
+        defaults = dict(lr=lr, betas=betas, eps=eps,
+                        weight_decay=weight_decay)
+        super().__init__(named_params, defaults, **ps_kwargs)
+
+    def _alloc_state(self):
+        flat = self.flat
+        if self.state_bits == 8:
+            self._m1 = ops.State8.zeros(flat.total, True, flat.device)
+            self._m2 = ops.State8.zeros(flat.total, False, flat.device)
+        else:
+            self._m1 = torch.zeros_like(flat.master)
+            self._m2 = torch.zeros_like(flat.master)
+        self._decay = None
+        if self._no_decay is not None:
+            decay = torch.ones(flat.total // ops.ACHUNK)
+            for name, p, o, n in flat.entries:
+                if self._no_decay(name, p):
+                    decay[o // ops.ACHUNK:-(-(o + n) // ops.ACHUNK)] = 0.0
+            self._decay = decay.to(flat.device)
+
+    def _apply_bucket(self, b):
+        g = self.param_groups[0]
+        flat = self.flat
+        count = self._bump(b)
+        beta1, beta2 = g["betas"]
+        if self.state_bits == 8:
+            m1, m2 = (m.span(b.start, b.end) for m in (self._m1, self._m2))
+        else:
+            m1, m2 = (m[b.start:b.end] for m in (self._m1, self._m2))
+        decay = None
+        if self._decay is not None:
+            decay = self._decay[b.start // ops.ACHUNK:b.end // ops.ACHUNK]
+        ops.fused_adamw(flat.master_view(b), m1, m2, flat.agg_view(b),
+                        self._param_out(b), lr=g["lr"], beta1=beta1,
+                        beta2=beta2, eps=g["eps"], wd=g["weight_decay"],
+                        step=count, decay=decay, offset=b.start,
+                        seed=self.seed)
+
+    def _state_tensors(self):
+        if self.state_bits == 8:
+            return {"exp_avg_codes": self._m1.codes,
+                    "exp_avg_scales": self._m1.scales,
+                    "exp_avg_sq_codes": self._m2.codes,
+                    "exp_avg_sq_scales": self._m2.scales}
+        return {"exp_avg": self._m1, "exp_avg_sq": self._m2}
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["state_bits"], sd["seed"] = self.state_bits, self.seed
+        return sd
+
+    def load_state_dict(self, sd):
+        if sd.get("state_bits") != self.state_bits:
+            raise ValueError(
+                f"checkpoint holds {sd.get('state_bits')}-bit AdamW states, "
+                f"this optimizer has {self.state_bits}-bit ones")
+        self.seed = sd["seed"]
+        super().load_state_dict(sd)

@@ -23,6 +23,7 @@ setup(
             sources=[
                 os.path.join(CSRC, "bindings.cpp"),
                 os.path.join(CSRC, "ps_kernels.hip"),
+                os.path.join(CSRC, "adamw_kernels.hip"),
                 os.path.join(CSRC, "bn_kernels.hip"),
                 os.path.join(CSRC, "ln_kernels.hip"),
                 os.path.join(CSRC, "ce_kernels.hip"),
@@ -31,7 +32,10 @@ setup(
             ],
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17"],
+                # no packed fp32 arithmetic: some of its forms have given
+                # wrong results on this hardware
+                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],
