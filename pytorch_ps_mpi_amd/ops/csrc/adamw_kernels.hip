@@ -67,10 +67,9 @@ __device__ __forceinline__ float aw_decode(uint32_t c, float scale) {
 //   up = expm1((e - lo) ln2/8) / (2^(1/8) - 1),  k = lo + (u < up).
 // The quotient: a times the reciprocal, put right by its own remainder.
 template <int TOP>
-__device__ __forceinline__ uint32_t aw_encode(float x, float s, float lift,
-                                              float inv, uint32_t r16) {
+__device__ __noinline__ uint32_t aw_code_exact(float a, float s, float inv,
+                                               uint32_t r16) {
 #pragma clang fp contract(off)
-  const float a = fabsf(x) * lift;
   float r = a * inv;
   r = __builtin_fmaf(__builtin_fmaf(-r, s, a), inv, r);
   const float e = (float)TOP + 8.0f * __builtin_amdgcn_logf(r);
@@ -83,8 +82,31 @@ __device__ __forceinline__ uint32_t aw_encode(float x, float s, float lift,
     if (TOP == 255) k = 1.0f;
     else k = u < __builtin_amdgcn_exp2f((e - 1.0f) * 0.125f) ? 1.0f : 0.0f;
   }
-  if (!(a > 0.0f)) k = 0.0f;
-  uint32_t c = (uint32_t)k;
+  return (uint32_t)k;
+}
+
+// The same code by a third of the instructions: quotient without its
+// correction, exp2 in place of expm1.  That moves e by at most one rounding
+// (2^-16) and up by 1.04 times that and 1.5e-6, 1.8e-5 together: where u is
+// that near to up, e that near to a whole number or under the lowest code
+// (about 1 of 10^4 values), the exact form decides.
+template <int TOP>
+__device__ __forceinline__ uint32_t aw_encode(float x, float s, float lift,
+                                              float inv, bool lifted,
+                                              uint32_t r16) {
+  const float a = fabsf(x);
+  const float e = fmaf(8.0f, __builtin_amdgcn_logf(a * inv), (float)TOP);
+  const float lo = floorf(e);
+  const float f = e - lo;
+  const float t = __builtin_amdgcn_exp2f(f * 0.125f);
+  // 65536 up - 0.5 against the 16 bits
+  const float d = fmaf(t, 65536.0f * 11.0487795f,
+                       -65536.0f * 11.0487795f - 0.5f) - (float)r16;
+  uint32_t c = (uint32_t)fminf(lo + (d > 0.0f ? 1.0f : 0.0f), (float)TOP);
+  const bool near = fabsf(d) < 1.4f || fabsf(f - 0.5f) > 0.49998f || e < 1.5f ||
+                    lifted;
+  if (!(a > 0.0f)) c = 0;
+  else if (near) c = aw_code_exact<TOP>(a * lift, s, inv, r16);
   if (TOP == 127 && x < 0.0f && c) c |= 128u;
   return c;
 }
@@ -107,8 +129,12 @@ __device__ __forceinline__ void aw_moments(const AwArgs& a, float g, float& m,
 __device__ __forceinline__ float aw_param(const AwArgs& a, float p, float m,
                                           float v, float lwd) {
   p = fmaf(-lwd, p, p);
-  const float d = fmaf(__builtin_amdgcn_sqrtf(v), a.inv_bc2_sqrt, a.eps);
-  return fmaf(-a.step_size, m / d, p);
+  // the square root instruction wants normal numbers
+  const float r = v < 1e-30f
+      ? __builtin_amdgcn_sqrtf(v * 1.2676506e30f) * 8.8817842e-16f
+      : __builtin_amdgcn_sqrtf(v);
+  const float d = fmaf(r, a.inv_bc2_sqrt, a.eps);
+  return fmaf(-a.step_size, m * __builtin_amdgcn_rcpf(d), p);
 }
 
 // OUT: 0 none, 1 bf16, 2 f32.  VEC: 16-byte accesses; else element by element
@@ -208,8 +234,8 @@ __device__ __forceinline__ void aw_chunk(const AwArgs& a, int64_t c, int lane) {
     for (int j = 0; j < 4; ++j) {
       const uint64_t e = e0 + j;
       const uint32_t r = aw_mix((uint32_t)e ^ aw_mix(a.key + (uint32_t)(e >> 32)));
-      mc |= aw_encode<127>(m[j], mx, ml, mi, r & 0xffffu) << (8 * j);
-      vc |= aw_encode<255>(v[j], vx, vl, vi, r >> 16) << (8 * j);
+      mc |= aw_encode<127>(m[j], mx, ml, mi, ml > 1.0f, r & 0xffffu) << (8 * j);
+      vc |= aw_encode<255>(v[j], vx, vl, vi, vl > 1.0f, r >> 16) << (8 * j);
     }
     if (VEC) {
       *(uint32_t*)(a.m8 + i0) = mc;
@@ -250,25 +276,28 @@ __global__ void __launch_bounds__(AW_BLOCK) k_fused_adamw(AwArgs a) {
   }
 }
 
+// 16 codes a lane: one 16-byte load.
 template <int TOP, typename T>
 __global__ void __launch_bounds__(AW_BLOCK)
 k_state8_values(const uint8_t* __restrict__ codes,
                 const float* __restrict__ scales, T* __restrict__ out,
                 int64_t n, int vec) {
-  const int64_t stride = (int64_t)gridDim.x * AW_BLOCK * 4;
-  for (int64_t i = ((int64_t)blockIdx.x * AW_BLOCK + threadIdx.x) * 4; i < n;
+  const int64_t stride = (int64_t)gridDim.x * AW_BLOCK * 16;
+  for (int64_t i = ((int64_t)blockIdx.x * AW_BLOCK + threadIdx.x) * 16; i < n;
        i += stride) {
     const float s = scales[i / AW_CHUNK];
-    if (vec && i + 4 <= n) {
-      const uint32_t c = *(const uint32_t*)(codes + i);
-      T o[4];
+    if (vec && i + 16 <= n) {
+      const uint4 c4 = *(const uint4*)(codes + i);
+      const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+      T o[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = (T)aw_decode<TOP>((c >> (8 * j)) & 255u, s);
-      if (sizeof(T) == 4) *(uint4*)(out + i) = *(uint4*)o;
-      else *(uint2*)(out + i) = *(uint2*)o;
+      for (int j = 0; j < 16; ++j)
+        o[j] = (T)aw_decode<TOP>((c[j / 4] >> (8 * (j & 3))) & 255u, s);
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T); ++j)
+        ((uint4*)(out + i))[j] = ((uint4*)o)[j];
     } else {
-      for (int j = 0; j < 4 && i + j < n; ++j)
+      for (int j = 0; j < 16 && i + j < n; ++j)
         out[i + j] = (T)aw_decode<TOP>(codes[i + j], s);
     }
   }
@@ -323,8 +352,8 @@ extern "C" int ps_state8_values(void* stream, const uint8_t* codes,
                                 int out_is_bf16, int is_signed, int64_t n) {
   if (n <= 0) return 0;
   hipStream_t s = (hipStream_t)stream;
-  const int grid = aw_grid((n + 4 * AW_BLOCK - 1) / (4 * AW_BLOCK));
-  const int vec = aw_al(codes, 4) && aw_al(out, out_is_bf16 ? 8 : 16);
+  const int grid = aw_grid((n + 16 * AW_BLOCK - 1) / (16 * AW_BLOCK));
+  const int vec = aw_al(codes, 16) && aw_al(out, 16);
   if (out_is_bf16) {
     auto o = (__hip_bfloat16*)out;
     if (is_signed)
