@@ -435,3 +435,4 @@ from . import ln  # noqa: E402,F401
 from . import ce  # noqa: E402,F401
 from . import attn  # noqa: E402,F401
 from . import linear  # noqa: E402,F401
+from . import rope  # noqa: E402,F401

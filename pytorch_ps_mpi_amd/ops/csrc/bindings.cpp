@@ -23,6 +23,18 @@ int ps_fused_adamw(void* stream, float* p, void* out, int out_kind,
                    float inv_bc2_sqrt, float eps, float gscale, uint32_t key);
 int ps_state8_values(void* stream, const uint8_t* codes, const float* scales,
                      void* out, int out_is_bf16, int is_signed, int64_t n);
+int ps_rope(void* stream, const void* q, const void* k, void* yq, void* yk,
+            const void* pos, int pos64, int dtype, const int64_t* strides,
+            int64_t B, int64_t N, int H, int KV, int D, int P,
+            const int* start, const double* rev, int inter, int backward);
+int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int backward);
+int ps_join_fwd(void* stream, void* const* t, float* const* stats, int bf16,
+                int64_t groups, int64_t rows, int64_t D, int layer,
+                int gate_kind, int64_t gate_step, float scale, float eps);
+int ps_join_bwd(void* stream, void* const* t, float* const* stats,
+                void* const* sums, float* part, int bf16, int64_t groups,
+                int64_t rows, int64_t D, int layer, int gate_kind,
+                int64_t gate_step, float scale);
 int ps_reduce_accum(void* stream, float* dst, const void** srcs, int nsrc,
                     int src_is_bf16, int64_t n, float scale, float beta);
 int ps_f32_to_bf16(void* stream, const float* src, void* dst, int64_t n);
@@ -121,6 +133,7 @@ void throw_on(int err, const char* what) {
   TORCH_CHECK(err != 9002, what,
               ": int8 payload/dst must be 8/16B-aligned (use the codec wire "
               "layout: scales padded to 16B before q)");
+  TORCH_CHECK(err != 9003, what, ": size out of the kernel's range");
   TORCH_CHECK(err == 0, what, ": hip error ", err);
 }
 
@@ -264,6 +277,146 @@ void state8_values(at::Tensor codes, at::Tensor scales, at::Tensor out,
                             scales.data_ptr<float>(), out.data_ptr(),
                             is_bf16(out), is_signed ? 1 : 0, n),
            "state8_values");
+}
+
+int float_kind(const at::Tensor& t, const char* name) {
+  const auto st = t.scalar_type();
+  TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || st == at::kFloat, name,
+              " must be bf16, fp16 or fp32");
+  return st == at::kBFloat16 ? 0 : st == at::kHalf ? 1 : 2;
+}
+
+void rope(at::Tensor q, at::Tensor k, at::Tensor yq, at::Tensor yk,
+          at::Tensor pos, std::vector<int64_t> start, at::Tensor rev,
+          bool inter, bool backward) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4, "q, k: 4-D on GPU");
+  TORCH_CHECK(q.stride(3) == 1 && k.stride(3) == 1, "unit last stride");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+                  q.size(3) == k.size(3) && k.scalar_type() == q.scalar_type(),
+              "q and k differ in B, N, D or type");
+  TORCH_CHECK(yq.sizes() == q.sizes() && yk.sizes() == k.sizes(), "out sizes");
+  check_flat(yq, q.scalar_type(), "yq");
+  check_flat(yk, q.scalar_type(), "yk");
+  for (const auto& t : {k, yq, yk, pos}) check_same_device(q, t, "rope input");
+  TORCH_CHECK(pos.dim() == 3 && pos.size(1) == q.size(0) &&
+                  pos.size(2) == q.size(1), "positions [axes, B, N]");
+  TORCH_CHECK(pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt,
+              "positions int32/int64");
+  TORCH_CHECK(rev.device().is_cpu() && rev.scalar_type() == at::kDouble &&
+                  rev.is_contiguous() && start.size() == 3, "rope plan");
+  const int P = (int)rev.numel();
+  int first[3];
+  int axes = 1;
+  for (int i = 0; i < 3; ++i) {
+    first[i] = (int)start[i];
+    axes += first[i] < P;
+  }
+  TORCH_CHECK(pos.size(0) >= axes, "a position for each axis");
+  const int64_t strides[9] = {q.stride(0), q.stride(1), q.stride(2),
+                              k.stride(0), k.stride(1), k.stride(2),
+                              pos.stride(0), pos.stride(1), pos.stride(2)};
+  const c10::DeviceGuard guard(q.device());
+  throw_on(ps_rope(cur_stream(q), q.data_ptr(), k.data_ptr(), yq.data_ptr(),
+                   yk.data_ptr(), pos.data_ptr(),
+                   pos.scalar_type() == at::kLong, float_kind(q, "q"), strides,
+                   q.size(0), q.size(1), (int)q.size(2), (int)k.size(2),
+                   (int)q.size(3), P, first, rev.data_ptr<double>(),
+                   inter ? 1 : 0, backward ? 1 : 0),
+           "rope");
+}
+
+// ---- norms before and after a block with its gate and residual ------------
+
+using OptTensors = std::vector<c10::optional<at::Tensor>>;
+
+// Pointers of `t`; entry i holds numel[i] elements of `like`'s type.
+void join_ptrs(const OptTensors& t, const std::vector<int64_t>& numel,
+               const at::Tensor& like, void** out) {
+  TORCH_CHECK(t.size() == numel.size(), "join: wrong number of tensors");
+  for (size_t i = 0; i < t.size(); ++i) {
+    out[i] = nullptr;
+    if (!t[i].has_value()) continue;
+    check_flat(*t[i], like.scalar_type(), "join tensor");
+    check_same_device(like, *t[i], "join tensor");
+    TORCH_CHECK(t[i]->numel() == numel[i], "join tensor ", i, " has ",
+                t[i]->numel(), " elements, expected ", numel[i]);
+    out[i] = t[i]->data_ptr();
+  }
+}
+
+void join_stats(const at::Tensor& stats, const at::Tensor& like, int64_t rows,
+                bool post, float** out) {
+  check_flat(stats, at::kFloat, "stats");
+  check_same_device(like, stats, "stats");
+  TORCH_CHECK(stats.numel() == (post ? 4 : 2) * rows, "stats size");
+  float* p = stats.data_ptr<float>();
+  for (int i = 0; i < 4; ++i) out[i] = i < 2 || post ? p + i * rows : nullptr;
+}
+
+int64_t join_gate(int64_t kind, int64_t step, int64_t groups, int64_t rows,
+                  int64_t D) {
+  TORCH_CHECK(kind >= 0 && kind <= 2 && (step == 0 || step == D), "gate kind");
+  return kind == 2 ? groups * rows * D : step ? groups * D : D;
+}
+
+int64_t join_blocks(int64_t groups, int64_t rows, int64_t D) {
+  return ps_join_blocks(groups, rows, D, 1);
+}
+
+// t: x, u, w, b, pw, pb, gate, y, h
+void join_fwd(OptTensors t, at::Tensor stats, int64_t groups, int64_t rows,
+              int64_t D, bool layer, int64_t gate_kind, int64_t gate_step,
+              double scale, double eps) {
+  TORCH_CHECK(t.size() == 9 && t[0] && t[1] && t[2] && t[7] && t[8],
+              "join_fwd: x, u, w, y, h wanted");
+  TORCH_CHECK(gate_kind == 0 || t[6], "join_fwd: gate wanted");
+  const at::Tensor& x = *t[0];
+  TORCH_CHECK(is_bf16(x) || x.scalar_type() == at::kFloat, "bf16 or fp32");
+  const int64_t n = groups * rows * D;
+  const int64_t ng = join_gate(gate_kind, gate_step, groups, rows, D);
+  void* p[9];
+  float* st[4];
+  join_ptrs(t, {n, n, D, D, D, D, ng, n, n}, x, p);
+  join_stats(stats, x, groups * rows, t[4].has_value(), st);
+  const c10::DeviceGuard guard(x.device());
+  throw_on(ps_join_fwd(cur_stream(x), p, st, is_bf16(x), groups, rows, D,
+                       layer ? 1 : 0, (int)gate_kind, gate_step, (float)scale,
+                       (float)eps),
+           "join_fwd");
+}
+
+// t: u, w, pw, pb, gate, y, dy, dh, dx, du, dgate; sums: dw, db, dgate, dpw,
+// dpb
+void join_bwd(OptTensors t, at::Tensor stats, OptTensors sums, at::Tensor part,
+              int64_t groups, int64_t rows, int64_t D, bool layer,
+              int64_t gate_kind, int64_t gate_step, double scale) {
+  TORCH_CHECK(t.size() == 11 && t[0] && t[1] && t[5] && t[8] && t[9],
+              "join_bwd: u, w, y, dx, du wanted");
+  TORCH_CHECK(gate_kind == 0 || t[4], "join_bwd: gate wanted");
+  const at::Tensor& u = *t[0];
+  TORCH_CHECK(is_bf16(u) || u.scalar_type() == at::kFloat, "bf16 or fp32");
+  const int64_t n = groups * rows * D;
+  const int64_t ng = join_gate(gate_kind, gate_step, groups, rows, D);
+  void *p[11], *s[5];
+  float* st[4];
+  join_ptrs(t, {n, D, D, D, ng, n, n, n, n, n, n}, u, p);
+  join_ptrs(sums, {D, D, ng, D, D}, u, s);
+  TORCH_CHECK((!s[3] && !s[4]) || p[2], "join_bwd: post sums without a post norm");
+  TORCH_CHECK((!s[2] && !p[10]) || gate_kind, "join_bwd: gate sums without a gate");
+  TORCH_CHECK(!s[2] || gate_kind == 1, "join_bwd: vector gate expected");
+  join_stats(stats, u, groups * rows, t[2].has_value(), st);
+  check_flat(part, at::kFloat, "part");
+  check_same_device(u, part, "part");
+  int64_t slots = 0;
+  for (void* q : s) slots += q != nullptr;
+  TORCH_CHECK(part.numel() >=
+                  groups * ps_join_blocks(groups, rows, D, 1) * slots * D,
+              "join_bwd: part too small");
+  const c10::DeviceGuard guard(u.device());
+  throw_on(ps_join_bwd(cur_stream(u), p, st, s, part.data_ptr<float>(),
+                       is_bf16(u), groups, rows, D, layer ? 1 : 0,
+                       (int)gate_kind, gate_step, (float)scale),
+           "join_bwd");
 }
 
 void reduce_accum(at::Tensor dst, std::vector<at::Tensor> srcs, double scale,
@@ -703,6 +856,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_adamw", &fused_adamw,
         "AdamW over packed fp32 buffers, states in 32 or 8 bits");
   m.def("state8_values", &state8_values, "values that 8-bit codes stand for");
+  m.def("rope", &rope, "rotary positions with several axes, q and k at once");
+  m.def("join_blocks", &join_blocks);
+  m.def("join_fwd", &join_fwd, "post norm, gate, residual, pre norm");
+  m.def("join_bwd", &join_bwd);
   m.def("reduce_accum", &reduce_accum, "dst = beta*dst + scale*sum(srcs)");
   m.def("f32_to_bf16", &f32_to_bf16, "flat cast");
   m.def("bf16_to_f32", &bf16_to_f32, "flat cast");

@@ -1,0 +1,475 @@
+// join_kernels.hip — what stands between two sublayers of a transformer block
+// (gfx950 / MI355X):
+//
+//   n = Post(u) (or u) ;  y = scale * x + gate * n ;  h = Norm(y)
+//
+// Norm and Post are layer norms or root-mean-square norms; the gate is absent,
+// one vector for all rows, one for each sample, or a whole tensor.
+//
+// Bound by HBM: the forward pass reads x, u and writes y, h; the backward pass
+// reads y, u, dy, dh and writes dx, du, everything else of a row stays in
+// registers.  A row belongs to one wave (D <= 1024) or one block (D <= 8192),
+// at most 16 elements a lane.  Means and variances in fp32, the variance about
+// the mean (two sums), h from the unrounded y; the backward pass takes the
+// rounded y, whose error of half a step is averaged like that of any input.
+//
+// Sums over rows (weights, biases, gate): each block keeps its rows' sums in
+// registers, writes them once, and a second kernel adds the blocks' parts in
+// fixed order.  No atomics: results repeat bit for bit.
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <cstdint>
+
+#define JN_MAXD 8192
+
+struct JoinArgs {
+  const void *x, *u, *w, *b, *pw, *pb, *gate;
+  void *y, *h;
+  float *my, *ry, *mu, *ru;            // statistics of the rows
+  const void *dy, *dh;                 // either may be null
+  void *dx, *du, *dgate;               // dgate: whole-tensor gate only
+  float* part;                         // [blocks][slots][D]
+  int slot_w, slot_b, slot_pw, slot_pb, slot_g, slots;
+  int64_t rows;                        // of a group
+  int nb;                              // blocks of a group
+  int D;
+  int layer;                           // 1: mean subtracted
+  int gate_kind;                       // 0 none, 1 one vector a group, 2 whole
+  int64_t gate_step;                   // from one group's vector to the next
+  float scale, eps, invD;
+};
+
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) JnVec { T v[VEC]; };
+
+__device__ __forceinline__ float jn_f(float v) { return v; }
+__device__ __forceinline__ float jn_f(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T jn_t(float v);
+template <> __device__ __forceinline__ float jn_t(float v) { return v; }
+template <> __device__ __forceinline__ __hip_bfloat16 jn_t(float v) { return __float2bfloat16(v); }
+
+// A lane's share of a row: EPT elements in vectors of VEC, TPR lanes a row.
+template <typename T, int VEC, int EPT, int TPR>
+struct JnRow {
+  static constexpr int CH = EPT / VEC;
+  JnVec<T, VEC> c[CH];
+  __device__ __forceinline__ static int at(int j, int lane) {
+    return ((j / VEC) * TPR + lane) * VEC + j % VEC;
+  }
+  // past the row's end: zeros
+  __device__ __forceinline__ void load(const void* p, int64_t off, int lane, int D) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e = (i * TPR + lane) * VEC;
+      if (e < D) {
+        c[i] = *(const JnVec<T, VEC>*)((const T*)p + off + e);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) c[i].v[j] = jn_t<T>(0.0f);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(void* p, int64_t off, int lane, int D) const {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e = (i * TPR + lane) * VEC;
+      if (e < D) *(JnVec<T, VEC>*)((T*)p + off + e) = c[i];
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return jn_f(c[j / VEC].v[j % VEC]); }
+  __device__ __forceinline__ void set(int j, float v) { c[j / VEC].v[j % VEC] = jn_t<T>(v); }
+};
+
+// Sums over the lanes of a row.  `red`: room for two rounds of a block's waves.
+template <int TPR>
+__device__ __forceinline__ float2 jn_sum2(float a, float b, float2* red, int& turn) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    a += __shfl_xor(a, d, 64);
+    b += __shfl_xor(b, d, 64);
+  }
+  if (TPR == 64) return make_float2(a, b);
+  constexpr int W = TPR / 64;
+  float2* r = red + turn * W;
+  turn ^= 1;
+  if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = make_float2(a, b);
+  __syncthreads();
+  a = b = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    a += r[i].x;
+    b += r[i].y;
+  }
+  return make_float2(a, b);
+}
+
+template <int TPR>
+__device__ __forceinline__ float jn_sum(float a, float2* red, int& turn) {
+  return jn_sum2<TPR>(a, 0.0f, red, turn).x;
+}
+
+// mean (0 for the rms kind) and 1/sqrt(variance + eps) of a row in f
+template <int EPT, int TPR, typename R>
+__device__ __forceinline__ void jn_stats(const JoinArgs& a, const float* f, int lane,
+                                         float& mean, float& rstd, float2* red, int& turn) {
+  mean = 0.0f;
+  if (a.layer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) s += f[j];
+    mean = jn_sum<TPR>(s, red, turn) * a.invD;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int j = 0; j < EPT; ++j) {
+    const float d = R::at(j, lane) < a.D ? f[j] - mean : 0.0f;
+    q = fmaf(d, d, q);
+  }
+  q = jn_sum<TPR>(q, red, turn);
+  rstd = 1.0f / sqrtf(fmaf(q, a.invD, a.eps));
+}
+
+template <typename T, int VEC, int EPT, int TPR, bool POST>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+k_join_fwd(const JoinArgs a) {
+  using R = JnRow<T, VEC, EPT, TPR>;
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;  // rows a block has in hand
+  __shared__ float2 red[2 * (TPR / 64)];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int group = blockIdx.x / a.nb, blk = blockIdx.x - group * a.nb;
+  const int D = a.D;
+  int turn = 0;
+  R w, b, pw, pb, gate;
+  w.load(a.w, 0, lane, D);
+  if (a.b) b.load(a.b, 0, lane, D);
+  if (POST) {
+    pw.load(a.pw, 0, lane, D);
+    if (a.pb) pb.load(a.pb, 0, lane, D);
+  }
+  if (a.gate_kind == 1) gate.load(a.gate, group * a.gate_step, lane, D);
+  for (int64_t i = (int64_t)blk * RPB + sub; i < a.rows; i += (int64_t)a.nb * RPB) {
+    const int64_t row = group * a.rows + i, off = row * D;
+    R x, u;
+    x.load(a.x, off, lane, D);
+    u.load(a.u, off, lane, D);
+    if (a.gate_kind == 2) gate.load(a.gate, off, lane, D);
+    float f[EPT];
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) f[j] = u.get(j);
+    if (POST) {
+      float m, r;
+      jn_stats<EPT, TPR, R>(a, f, lane, m, r, red, turn);
+      if (lane == 0) {
+        a.mu[row] = m;
+        a.ru[row] = r;
+      }
+#pragma unroll
+      for (int j = 0; j < EPT; ++j)
+        f[j] = fmaf((f[j] - m) * r, pw.get(j), a.pb ? pb.get(j) : 0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) {
+      const float g = a.gate_kind ? gate.get(j) * f[j] : f[j];
+      f[j] = R::at(j, lane) < D ? fmaf(a.scale, x.get(j), g) : 0.0f;
+      x.set(j, f[j]);
+    }
+    x.store(a.y, off, lane, D);
+    float m, r;
+    jn_stats<EPT, TPR, R>(a, f, lane, m, r, red, turn);
+    if (lane == 0) {
+      a.my[row] = m;
+      a.ry[row] = r;
+    }
+#pragma unroll
+    for (int j = 0; j < EPT; ++j)
+      u.set(j, fmaf((f[j] - m) * r, w.get(j), a.b ? b.get(j) : 0.0f));
+    u.store(a.h, off, lane, D);
+  }
+}
+
+// This block's sums of one slot, to its part: the RPB rows in hand are added
+// through LDS in fixed order.
+template <int VEC, int EPT, int TPR, typename R>
+__device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int slot,
+                                        int lane, int sub, float* lds) {
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  if (slot < 0) return;
+  float* out = a.part + ((int64_t)blockIdx.x * a.slots + slot) * a.D;
+  if (RPB == 1) {
+#pragma unroll
+    for (int j = 0; j < EPT; ++j)
+      if (R::at(j, lane) < a.D) out[R::at(j, lane)] = acc[j];
+    return;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < EPT; ++j) lds[sub * EPT * TPR + R::at(j, lane)] = acc[j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.D; e += 256) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < RPB; ++k) s += lds[k * EPT * TPR + e];
+    out[e] = s;
+  }
+}
+
+template <typename T, int VEC, int EPT, int TPR, bool POST>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+k_join_bwd(const JoinArgs a) {
+  using R = JnRow<T, VEC, EPT, TPR>;
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float2 red[2 * (TPR / 64)];
+  __shared__ float lds[RPB == 1 ? 1 : RPB * EPT * TPR];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int group = blockIdx.x / a.nb, blk = blockIdx.x - group * a.nb;
+  const int D = a.D;
+  int turn = 0;
+  R w, pw, pb, gate;
+  float aw[EPT], ab[EPT], ag[EPT], apw[POST ? EPT : 1], apb[POST ? EPT : 1];
+#pragma unroll
+  for (int j = 0; j < EPT; ++j) {
+    aw[j] = ab[j] = ag[j] = 0.0f;
+    if (POST) apw[j] = apb[j] = 0.0f;
+  }
+  w.load(a.w, 0, lane, D);
+  if (POST) {
+    pw.load(a.pw, 0, lane, D);
+    if (a.pb) pb.load(a.pb, 0, lane, D);
+  }
+  if (a.gate_kind == 1) gate.load(a.gate, group * a.gate_step, lane, D);
+  for (int64_t i = (int64_t)blk * RPB + sub; i < a.rows; i += (int64_t)a.nb * RPB) {
+    const int64_t row = group * a.rows + i, off = row * D;
+    R y, u, dy, dh;
+    if (a.dh) {
+      y.load(a.y, off, lane, D);
+      dh.load(a.dh, off, lane, D);
+    }
+    u.load(a.u, off, lane, D);
+    if (a.dy) dy.load(a.dy, off, lane, D);
+    if (a.gate_kind == 2) gate.load(a.gate, off, lane, D);
+    float t[EPT];  // the whole gradient of y
+    if (a.dh) {
+      const float m = a.my[row], r = a.ry[row];
+      float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int j = 0; j < EPT; ++j) {
+        const float xh = (y.get(j) - m) * r, g = dh.get(j);
+        aw[j] = fmaf(g, xh, aw[j]);
+        ab[j] += g;
+        const float k = g * w.get(j);
+        s1 += k;
+        s2 = fmaf(k, xh, s2);
+      }
+      const float2 s = jn_sum2<TPR>(s1, s2, red, turn);
+      const float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
+#pragma unroll
+      for (int j = 0; j < EPT; ++j) {
+        const float xh = (y.get(j) - m) * r;
+        t[j] = r * (fmaf(dh.get(j), w.get(j), -c1) - xh * c2);
+        if (a.dy) t[j] += dy.get(j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPT; ++j) t[j] = a.dy ? dy.get(j) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) y.set(j, a.scale * t[j]);
+    y.store(a.dx, off, lane, D);
+    float m = 0.0f, r = 1.0f, s1 = 0.0f, s2 = 0.0f;
+    if (POST) {
+      m = a.mu[row];
+      r = a.ru[row];
+    }
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) {
+      const float uh = POST ? (u.get(j) - m) * r : u.get(j);
+      if (a.gate_kind) {
+        const float n = POST ? fmaf(uh, pw.get(j), a.pb ? pb.get(j) : 0.0f) : uh;
+        const float g = t[j] * n;
+        ag[j] += g;
+        dy.set(j, g);
+        t[j] *= gate.get(j);
+      }
+      if (POST) {
+        apw[j] = fmaf(t[j], uh, apw[j]);
+        apb[j] += t[j];
+        t[j] *= pw.get(j);
+        s1 += t[j];
+        s2 = fmaf(t[j], uh, s2);
+      }
+    }
+    if (a.dgate) dy.store(a.dgate, off, lane, D);
+    if (POST) {
+      const float2 s = jn_sum2<TPR>(s1, s2, red, turn);
+      const float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
+#pragma unroll
+      for (int j = 0; j < EPT; ++j)
+        t[j] = r * (t[j] - c1 - (u.get(j) - m) * r * c2);
+    }
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) u.set(j, t[j]);
+    u.store(a.du, off, lane, D);
+  }
+  // lanes past the row's end held w = pw = 0 and are not written
+  jn_part<VEC, EPT, TPR, R>(a, aw, a.slot_w, lane, sub, lds);
+  jn_part<VEC, EPT, TPR, R>(a, ab, a.slot_b, lane, sub, lds);
+  jn_part<VEC, EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
+  if (POST) {
+    jn_part<VEC, EPT, TPR, R>(a, apw, a.slot_pw, lane, sub, lds);
+    jn_part<VEC, EPT, TPR, R>(a, apb, a.slot_pb, lane, sub, lds);
+  }
+}
+
+struct JoinSums {
+  void* out[5];     // by slot
+  const float* part;
+  int slots, slot_g, groups, nb, D;
+};
+
+// out[slot][d] = sum over blocks of part[block][slot][d]; the gate's slot one
+// sum for each group.  64 columns and 16 ranges of blocks a thread block.
+template <typename T>
+__global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
+  __shared__ float lds[16][64];
+  const int col = threadIdx.x & 63, rg = threadIdx.x >> 6;
+  const int d = blockIdx.x * 64 + col;
+  // y: first the slots summed over all blocks, then the gate's groups
+  const bool each = a.slot_g >= 0 && a.groups > 1;
+  const int whole = a.slots - (each ? 1 : 0);
+  int slot, first, count, g = 0;
+  if ((int)blockIdx.y < whole) {
+    slot = blockIdx.y;
+    if (each && slot >= a.slot_g) ++slot;
+    first = 0;
+    count = a.groups * a.nb;
+  } else {
+    slot = a.slot_g;
+    g = blockIdx.y - whole;
+    first = g * a.nb;
+    count = a.nb;
+  }
+  float s = 0.0f;
+  if (d < a.D)
+    for (int i = rg; i < count; i += 16)
+      s += a.part[((int64_t)(first + i) * a.slots + slot) * a.D + d];
+  lds[rg][col] = s;
+  __syncthreads();
+  if (rg == 0 && d < a.D) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += lds[i][col];
+    ((T*)a.out[slot])[(int64_t)g * a.D + d] = jn_t<T>(s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+static inline int jn_rpb(int D) { return D <= 1024 ? 4 : 1; }
+
+template <typename T, int VEC, bool BWD, bool POST>
+static void jn_launch(hipStream_t s, int grid, const JoinArgs& a) {
+#define JN_GO(EPT, TPR)                                                        \
+  do {                                                                         \
+    if (BWD)                                                                   \
+      hipLaunchKernelGGL((k_join_bwd<T, VEC, EPT, TPR, POST>), dim3(grid),     \
+                         dim3(TPR < 256 ? 256 : TPR), 0, s, a);                \
+    else                                                                       \
+      hipLaunchKernelGGL((k_join_fwd<T, VEC, EPT, TPR, POST>), dim3(grid),     \
+                         dim3(TPR < 256 ? 256 : TPR), 0, s, a);                \
+  } while (0)
+  if (a.D <= 512) JN_GO(8, 64);
+  else if (a.D <= 1024) JN_GO(16, 64);
+  else if (a.D <= 2048) JN_GO(8, 256);
+  else if (a.D <= 4096) JN_GO(16, 256);
+  else JN_GO(16, 512);
+#undef JN_GO
+}
+
+template <typename T, bool BWD>
+static void jn_pick(hipStream_t s, int grid, const JoinArgs& a, bool vec) {
+  constexpr int V = 16 / sizeof(T);
+  const bool post = a.pw != nullptr;
+  if (vec && post) jn_launch<T, V, BWD, true>(s, grid, a);
+  else if (vec) jn_launch<T, V, BWD, false>(s, grid, a);
+  else if (post) jn_launch<T, 1, BWD, true>(s, grid, a);
+  else jn_launch<T, 1, BWD, false>(s, grid, a);
+}
+
+// Blocks of a group: the backward kernel's registers let 512 blocks be on the
+// chip at once; more would only write more parts.
+extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D,
+                                  int backward) {
+  const int64_t most = (backward ? 512 : 2048) / groups;
+  int64_t nb = (rows + jn_rpb((int)D) - 1) / jn_rpb((int)D);
+  if (nb > most) nb = most;
+  return nb < 1 ? 1 : nb;
+}
+
+static int jn_check(const JoinArgs& a, int64_t groups) {
+  if (a.D < 1 || a.D > JN_MAXD || groups * a.nb > 0x7fffffff) return 9003;
+  return 0;
+}
+
+static bool jn_vec(const void* const* p, int n, int D, int bf16) {
+  bool ok = D % (bf16 ? 8 : 4) == 0;
+  for (int i = 0; i < n; ++i) ok = ok && ((uintptr_t)p[i] & 15) == 0;
+  return ok;
+}
+
+// t: x, u, w, b, pw, pb, gate, y, h;  stats: my, ry, mu, ru
+extern "C" int ps_join_fwd(void* stream, void* const* t, float* const* stats,
+                           int bf16, int64_t groups, int64_t rows, int64_t D,
+                           int layer, int gate_kind, int64_t gate_step,
+                           float scale, float eps) {
+  if (groups <= 0 || rows <= 0) return 0;
+  JoinArgs a{};
+  a.x = t[0]; a.u = t[1]; a.w = t[2]; a.b = t[3]; a.pw = t[4]; a.pb = t[5];
+  a.gate = t[6]; a.y = t[7]; a.h = t[8];
+  a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
+  a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
+  a.gate_step = gate_step; a.scale = scale; a.eps = eps; a.invD = 1.0f / (float)D;
+  a.nb = (int)ps_join_blocks(groups, rows, D, 0);
+  if (int e = jn_check(a, groups)) return e;
+  const bool vec = jn_vec((const void* const*)t, 9, (int)D, bf16);
+  const int grid = (int)(groups * a.nb);
+  if (bf16) jn_pick<__hip_bfloat16, false>((hipStream_t)stream, grid, a, vec);
+  else jn_pick<float, false>((hipStream_t)stream, grid, a, vec);
+  return (int)hipGetLastError();
+}
+
+// t: u, w, pw, pb, gate, y, dy, dh, dx, du, dgate (whole tensor);
+// sums: dw, db, dgate (vectors), dpw, dpb — null where not wanted.
+extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
+                           void* const* sums, float* part, int bf16,
+                           int64_t groups, int64_t rows, int64_t D, int layer,
+                           int gate_kind, int64_t gate_step, float scale) {
+  if (groups <= 0 || rows <= 0) return 0;
+  JoinArgs a{};
+  a.u = t[0]; a.w = t[1]; a.pw = t[2]; a.pb = t[3]; a.gate = t[4]; a.y = t[5];
+  a.dy = t[6]; a.dh = t[7]; a.dx = t[8]; a.du = t[9]; a.dgate = t[10];
+  a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
+  a.part = part;
+  a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
+  a.gate_step = gate_step; a.scale = scale; a.invD = 1.0f / (float)D;
+  a.nb = (int)ps_join_blocks(groups, rows, D, 1);
+  if (int e = jn_check(a, groups)) return e;
+  JoinSums q{};
+  int* slot[5] = {&a.slot_w, &a.slot_b, &a.slot_g, &a.slot_pw, &a.slot_pb};
+  for (int i = 0; i < 5; ++i) {
+    *slot[i] = sums[i] ? a.slots : -1;
+    if (sums[i]) q.out[a.slots++] = sums[i];
+  }
+  const bool vec = jn_vec((const void* const*)t, 11, (int)D, bf16);
+  const int grid = (int)(groups * a.nb);
+  hipStream_t s = (hipStream_t)stream;
+  if (bf16) jn_pick<__hip_bfloat16, true>(s, grid, a, vec);
+  else jn_pick<float, true>(s, grid, a, vec);
+  if (int e = (int)hipGetLastError()) return e;
+  if (a.slots == 0) return 0;
+  q.part = part; q.slots = a.slots; q.slot_g = a.slot_g;
+  q.groups = (int)groups; q.nb = a.nb; q.D = (int)D;
+  const int gy = a.slots + (a.slot_g >= 0 && groups > 1 ? (int)groups - 1 : 0);
+  const dim3 sg((unsigned)((D + 63) / 64), (unsigned)gy);
+  if (bf16) hipLaunchKernelGGL((k_join_sum<__hip_bfloat16>), sg, dim3(1024), 0, s, q);
+  else hipLaunchKernelGGL((k_join_sum<float>), sg, dim3(1024), 0, s, q);
+  return (int)hipGetLastError();
+}

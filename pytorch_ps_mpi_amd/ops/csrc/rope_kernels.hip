@@ -1,0 +1,184 @@
+// rope_kernels.hip — rotary positions with several axes (gfx950 / MI355X).
+//
+// A head's first 2P elements are P pairs; each pair belongs to one axis (time,
+// height, width) and turns by  position[axis] * freq[pair]:
+//   (a, b) -> (a cos - b sin, a sin + b cos);   backward: the turn by -angle.
+// Elements from 2P on pass through.
+//
+// The angle is taken in 64 bits as a number of revolutions, of which only the
+// fraction goes on (a position of a million in 32 bits would be 0.06 rad off);
+// it is computed once for a token and pair and used by all heads through LDS.
+// Bound by HBM: q and k are read once and written once.  The frequencies
+// travel in the kernel's arguments: no table lives on the device.
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <cstdint>
+
+#define RP_BLOCK 256
+#define RP_MAXP 256
+#define RP_TOK 4
+
+struct RopeTensor {
+  const void* x;
+  void* y;            // contiguous [B, N, H, D]
+  int64_t sB, sN, sH; // strides of x in elements
+  int H;
+};
+
+struct RopeArgs {
+  RopeTensor t[2];    // q, k
+  const void* pos;
+  int64_t pA, pB, pN; // strides of pos
+  int pos64;
+  int64_t rows;       // B * N
+  int N, D, P;
+  int start[4];       // first pair of axis 1, 2, 3 (P where there is none)
+  float sign;         // -1: backward
+  double rev[RP_MAXP];// revolutions for a position of 1
+};
+
+template <typename T> __device__ __forceinline__ float rp_f(T v) { return (float)v; }
+template <> __device__ __forceinline__ float rp_f(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float rp_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T rp_t(float v) { return (T)v; }
+template <> __device__ __forceinline__ __hip_bfloat16 rp_t(float v) { return __float2bfloat16(v); }
+template <> __device__ __forceinline__ __half rp_t(float v) { return __float2half(v); }
+
+// 16 bytes of T
+template <typename T> struct alignas(16) RpVec { T v[16 / sizeof(T)]; };
+
+__device__ __forceinline__ void rp_angles(const RopeArgs& a, int64_t row0,
+                                          int toks, float2* cs) {
+  for (int i = threadIdx.x; i < toks * a.P; i += RP_BLOCK) {
+    const int t = i / a.P, p = i - t * a.P;
+    const int64_t row = row0 + t;
+    const int64_t b = row / a.N, n = row - b * a.N;
+    const int axis = (p >= a.start[0]) + (p >= a.start[1]) + (p >= a.start[2]);
+    const int64_t at = axis * a.pA + b * a.pB + n * a.pN;
+    const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at]
+                               : (double)((const int32_t*)a.pos)[at];
+    const double r = pos * a.rev[p];
+    float s, c;
+    sincospif((float)(2.0 * (r - rint(r))), &s, &c);
+    cs[i] = make_float2(c, a.sign * s);
+  }
+}
+
+// VEC elements of 16 bytes at once; VEC == 1: any size and alignment.
+// Half-split: item c holds pairs [c*VEC, c*VEC+VEC), that is two vectors.
+// Interleaved: item c holds elements [c*VEC, ...), VEC/2 pairs.
+template <typename T, int VEC, bool INTER>
+__global__ void __launch_bounds__(RP_BLOCK) k_rope(const RopeArgs a) {
+  extern __shared__ float2 cs[];
+  const int64_t row0 = (int64_t)blockIdx.x * RP_TOK;
+  const int toks = (int)min((int64_t)RP_TOK, a.rows - row0);
+  rp_angles(a, row0, toks, cs);
+  __syncthreads();
+  const int P = a.P, D = a.D;
+  const int turn = INTER ? (VEC == 1 ? P : 2 * P / VEC) : P / VEC;
+  const int rest = (D - 2 * P) / VEC;  // items that pass through
+  const int per = turn + rest;
+  const int heads = a.t[0].H + a.t[1].H;
+  const int total = toks * heads * per;
+  for (int i = threadIdx.x; i < total; i += RP_BLOCK) {
+    const int th = i / per, c = i - th * per;
+    const int t = th / heads;
+    int h = th - t * heads;
+    const bool isk = h >= a.t[0].H;
+    const RopeTensor& w = a.t[isk];
+    if (isk) h -= a.t[0].H;
+    const int64_t row = row0 + t;
+    const int64_t b = row / a.N, n = row - b * a.N;
+    const T* x = (const T*)w.x + b * w.sB + n * w.sN + h * w.sH;
+    T* y = (T*)w.y + (row * w.H + h) * D;
+    const float2* tc = cs + t * P;
+    if (c >= turn) {
+      const int e = 2 * P + (c - turn) * VEC;
+      if (VEC == 1) y[e] = x[e];
+      else *(RpVec<T>*)(y + e) = *(const RpVec<T>*)(x + e);
+    } else if (VEC == 1) {
+      const int ia = INTER ? 2 * c : c, ib = INTER ? 2 * c + 1 : P + c;
+      const float va = rp_f(x[ia]), vb = rp_f(x[ib]);
+      const float2 k = tc[c];
+      y[ia] = rp_t<T>(va * k.x - vb * k.y);
+      y[ib] = rp_t<T>(va * k.y + vb * k.x);
+    } else if (INTER) {
+      const RpVec<T> v = *(const RpVec<T>*)(x + c * VEC);
+      RpVec<T> o;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 k = tc[c * (VEC / 2) + j / 2];
+        const float va = rp_f(v.v[j]), vb = rp_f(v.v[j + 1]);
+        o.v[j] = rp_t<T>(va * k.x - vb * k.y);
+        o.v[j + 1] = rp_t<T>(va * k.y + vb * k.x);
+      }
+      *(RpVec<T>*)(y + c * VEC) = o;
+    } else {
+      const RpVec<T> u = *(const RpVec<T>*)(x + c * VEC);
+      const RpVec<T> v = *(const RpVec<T>*)(x + P + c * VEC);
+      RpVec<T> o, q;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 k = tc[c * VEC + j];
+        const float va = rp_f(u.v[j]), vb = rp_f(v.v[j]);
+        o.v[j] = rp_t<T>(va * k.x - vb * k.y);
+        q.v[j] = rp_t<T>(va * k.y + vb * k.x);
+      }
+      *(RpVec<T>*)(y + c * VEC) = o;
+      *(RpVec<T>*)(y + P + c * VEC) = q;
+    }
+  }
+}
+
+template <typename T>
+static void rp_launch(hipStream_t s, const RopeArgs& a, bool vec, bool inter) {
+  constexpr int V = 16 / sizeof(T);
+  const int grid = (int)((a.rows + RP_TOK - 1) / RP_TOK);
+  const size_t lds = (size_t)RP_TOK * a.P * sizeof(float2);
+  if (vec && inter)
+    hipLaunchKernelGGL((k_rope<T, V, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+  else if (vec)
+    hipLaunchKernelGGL((k_rope<T, V, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+  else if (inter)
+    hipLaunchKernelGGL((k_rope<T, 1, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+  else
+    hipLaunchKernelGGL((k_rope<T, 1, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+}
+
+// strides: q's B, N, H, k's B, N, H, pos's axis, B, N.  dtype: 0 bf16, 1 fp16,
+// 2 fp32.  rev: revolutions a position for each of P pairs (host memory).
+extern "C" int ps_rope(void* stream, const void* q, const void* k, void* yq,
+                       void* yk, const void* pos, int pos64, int dtype,
+                       const int64_t* strides, int64_t B, int64_t N, int H,
+                       int KV, int D, int P, const int* start,
+                       const double* rev, int inter, int backward) {
+  const int64_t rows = B * N;
+  if (rows <= 0) return 0;
+  if (P < 1 || P > RP_MAXP || 2 * P > D ||
+      (rows + RP_TOK - 1) / RP_TOK > 0x7fffffff || N > 0x7fffffff ||
+      (int64_t)RP_TOK * ((int64_t)H + KV) * D > 0x7fffffff)
+    return 9003;
+  RopeArgs a;
+  a.t[0] = {q, yq, strides[0], strides[1], strides[2], H};
+  a.t[1] = {k, yk, strides[3], strides[4], strides[5], KV};
+  a.pos = pos;
+  a.pA = strides[6]; a.pB = strides[7]; a.pN = strides[8];
+  a.pos64 = pos64;
+  a.rows = rows;
+  a.N = (int)N; a.D = D; a.P = P;
+  for (int i = 0; i < 3; ++i) a.start[i] = start[i];
+  a.sign = backward ? -1.0f : 1.0f;
+  for (int i = 0; i < P; ++i) a.rev[i] = rev[i];
+  const int V = dtype == 2 ? 4 : 8;
+  bool vec = D % V == 0 && (inter ? 2 * P : P) % V == 0;
+  for (int i = 0; i < 6; ++i) vec = vec && strides[i] % V == 0;
+  for (const void* p : {q, k, (const void*)yq, (const void*)yk})
+    vec = vec && ((uintptr_t)p & 15) == 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == 0) rp_launch<__hip_bfloat16>(s, a, vec, inter);
+  else if (dtype == 1) rp_launch<__half>(s, a, vec, inter);
+  else rp_launch<float>(s, a, vec, inter);
+  return (int)hipGetLastError();
+}

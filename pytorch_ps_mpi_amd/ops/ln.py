@@ -12,7 +12,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import HAVE_EXT, _EXT
+from . import HAVE_EXT, _EXT, _require_ext
 
 
 class _FusedLN(torch.autograd.Function):
@@ -58,3 +58,146 @@ class FusedLayerNorm(nn.LayerNorm):
             return _FusedLN.apply(x, self.weight, self.bias, self.eps)
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias,
                             self.eps)
+
+
+# ---------------------------------------------------------------------------
+# norms before and after a block with its gate and residual scale
+# ---------------------------------------------------------------------------
+
+MAX_JOIN_DIM = 8192
+
+
+def _norm_plain(f, w, b, kind, eps):
+    if kind == "layer":
+        f = f - f.mean(-1, keepdim=True)
+    f = f * torch.rsqrt((f * f).mean(-1, keepdim=True) + eps) * w.to(f.dtype)
+    return f if b is None else f + b.to(f.dtype)
+
+
+def _join_plain(x, u, w, b, gate, pw, pb, scale, eps, kind):
+    t = torch.float64 if x.dtype == torch.float64 else torch.float32
+    n = u.to(t)
+    if pw is not None:
+        n = _norm_plain(n, pw, pb, kind, eps)
+    if gate is not None:
+        n = n * gate.to(t)
+    y = x.to(t) * scale + n
+    return y.to(x.dtype), _norm_plain(y, w, b, kind, eps).to(x.dtype)
+
+
+class _GatedResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, u, w, b, gate, pw, pb, scale, eps, kind, groups,
+                gate_kind):
+        D = x.shape[-1]
+        rows = x.numel() // D // groups
+        x, u, w, b, gate, pw, pb = (
+            None if t is None else t.contiguous()
+            for t in (x, u, w, b, gate, pw, pb))
+        y, h = torch.empty_like(x), torch.empty_like(x)
+        stats = torch.empty(4 if pw is not None else 2, groups * rows,
+                            dtype=torch.float32, device=x.device)
+        layer = kind == "layer"
+        step = D if gate_kind == 1 and groups > 1 else 0
+        _EXT.join_fwd([x, u, w, b, pw, pb, gate, y, h], stats, groups, rows, D,
+                      layer, gate_kind, step, scale, eps)
+        ctx.save_for_backward(y, u, w, gate, pw, pb, stats)
+        ctx.b_dtype = None if b is None else b.dtype
+        ctx.cfg = (groups, rows, D, layer, gate_kind, step, scale)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    def backward(ctx, dy, dh):
+        y, u, w, gate, pw, pb, stats = ctx.saved_tensors
+        groups, rows, D, layer, gate_kind, step, scale = ctx.cfg
+        need = dict(zip(("x", "u", "w", "b", "gate", "pw", "pb"),
+                        ctx.needs_input_grad))
+        dy, dh = (None if t is None else t.contiguous() for t in (dy, dh))
+        dx, du = torch.empty_like(y), torch.empty_like(u)
+
+        def like(t, wanted):
+            return torch.empty_like(t) if wanted and t is not None else None
+
+        # without dh the last norm's parameters get no gradient
+        dw = like(w, need["w"] and dh is not None)
+        db = None
+        if need["b"] and ctx.b_dtype is not None and dh is not None:
+            db = torch.empty_like(w)
+        dgate = like(gate, need["gate"])
+        dpw, dpb = like(pw, need["pw"]), like(pb, need["pb"])
+        whole = gate_kind == 2
+        sums = [dw, db, None if whole else dgate, dpw, dpb]
+        if dy is not None or dh is not None:
+            nsum = sum(t is not None for t in sums)
+            part = torch.empty(
+                groups * _EXT.join_blocks(groups, rows, D) * nsum * D,
+                dtype=torch.float32, device=y.device)
+            _EXT.join_bwd([u, w, pw, pb, gate, y, dy, dh, dx, du,
+                           dgate if whole else None], stats, sums, part,
+                          groups, rows, D, layer, gate_kind, step, scale)
+        else:
+            return (None,) * 12
+        return (dx if need["x"] else None, du if need["u"] else None, dw, db,
+                dgate, dpw, dpb, None, None, None, None, None)
+
+
+def fused_gated_residual(x, u, weight, bias=None, *, gate=None,
+                         post_weight=None, post_bias=None, scale=1.0,
+                         eps=1e-5, kind="layer"):
+    """A sublayer's end and the next one's beginning in one pass:
+
+        n = Post(u) if post_weight is given, else u
+        y = scale * x + gate * n          (the residual stream)
+        h = Norm(y)                       (input of the next sublayer)
+
+    Returns (y, h).  x, u: [..., D] of one type; ``weight``/``bias`` and
+    ``post_weight``/``post_bias``: [D] of that type; ``kind``: "layer" or "rms"
+    for both norms.  ``gate``: None, [D], [B, 1, D] for x of [B, T, D], or x's
+    shape.  The norm is taken of y before its rounding.
+
+    GPU: HIP kernels (ops/csrc/join_kernels.hip) for bf16 and fp32, D up to
+    8192; other types or sizes raise.  CPU: plain torch, the oracle.
+    """
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"kind must be 'layer' or 'rms', got {kind!r}")
+    if x.dim() < 1 or x.shape != u.shape:
+        raise ValueError(f"x {tuple(x.shape)} and u {tuple(u.shape)} must "
+                         "have one shape")
+    D = x.shape[-1]
+    if D < 1:
+        raise ValueError("rows must have at least one element")
+    if post_bias is not None and post_weight is None:
+        raise ValueError("post_bias needs post_weight")
+    for name, t in (("weight", weight), ("bias", bias),
+                    ("post_weight", post_weight), ("post_bias", post_bias)):
+        if t is not None and tuple(t.shape) != (D,):
+            raise ValueError(f"{name} must be [{D}], got {tuple(t.shape)}")
+    for name, t in (("u", u), ("weight", weight), ("bias", bias),
+                    ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("gate", gate)):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{name} must have x's type and device")
+    groups, gate_kind = 1, 0
+    if gate is not None:
+        if tuple(gate.shape) == (D,):
+            gate_kind = 1
+        elif gate.shape == x.shape:
+            gate_kind = 2
+        elif x.dim() == 3 and tuple(gate.shape) == (x.shape[0], 1, D):
+            gate_kind, groups = 1, x.shape[0]
+        else:
+            raise ValueError(
+                f"gate must be [{D}], [B, 1, {D}] or x's shape, got "
+                f"{tuple(gate.shape)}")
+    if _require_ext(x) and x.numel():
+        if x.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("fused_gated_residual on GPU: bf16 or fp32")
+        if D > MAX_JOIN_DIM:
+            raise ValueError(f"fused_gated_residual on GPU: rows of at most "
+                             f"{MAX_JOIN_DIM}, got {D}")
+        return _GatedResidual.apply(x, u, weight, bias, gate, post_weight,
+                                    post_bias, float(scale), float(eps), kind,
+                                    groups, gate_kind)
+    return _join_plain(x, u, weight, bias, gate, post_weight, post_bias,
+                       scale, eps, kind)

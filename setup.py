@@ -24,6 +24,8 @@ setup(
                 os.path.join(CSRC, "bindings.cpp"),
                 os.path.join(CSRC, "ps_kernels.hip"),
                 os.path.join(CSRC, "adamw_kernels.hip"),
+                os.path.join(CSRC, "join_kernels.hip"),
+                os.path.join(CSRC, "rope_kernels.hip"),
                 os.path.join(CSRC, "bn_kernels.hip"),
                 os.path.join(CSRC, "ln_kernels.hip"),
                 os.path.join(CSRC, "ce_kernels.hip"),
