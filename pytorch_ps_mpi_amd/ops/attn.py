@@ -10,6 +10,10 @@ Two in-tree implementations, selected by PS_AMD_ATTN:
 Shape contract for the fused paths: [B, H, N, D] bf16 contiguous, D == 64
 (GPT-2-small and ViT-B/16 head dim).  Anything else falls back to torch
 SDPA.
+
+``fused_window_sdpa`` is causal attention with a sliding window and first
+tokens that stay visible (ops/csrc/window_attn_kernels.hip): grouped heads,
+D 64 or 128, padded batches.
 """
 
 from __future__ import annotations
@@ -20,7 +24,7 @@ import os
 import torch
 import torch.nn.functional as F
 
-from . import HAVE_EXT, _EXT
+from . import HAVE_EXT, _EXT, _require_ext
 
 
 def _impl():
@@ -127,3 +131,123 @@ def fused_sdpa(q, k, v, is_causal=False):
         return _FusedSDPA.apply(q.contiguous(), k.contiguous(),
                                 v.contiguous(), bool(is_causal), mfma)
     return F.scaled_dot_product_attention(q, k, v, is_causal=is_causal)
+
+
+# ---------------------------------------------------------------------------
+# sliding window with first tokens that stay visible
+# ---------------------------------------------------------------------------
+
+def _window_plain(q, k, v, window, sinks, lengths, scale):
+    """The whole score matrix in fp32 (fp64 for fp64): oracle, and the path of
+    types and head sizes that have no kernel."""
+    B, H, N, D = q.shape
+    G = H // k.shape[1]
+    t = torch.float64 if q.dtype == torch.float64 else torch.float32
+    kf = k.to(t).repeat_interleave(G, 1)
+    vf = v.to(t).repeat_interleave(G, 1)
+    i = torch.arange(N, device=q.device)[:, None]
+    j = torch.arange(N, device=q.device)[None]
+    vis = ((j <= i) & ((i - j < window) | (j < sinks)))[None]
+    if lengths is not None:
+        n = lengths.long().clamp(0, N)[:, None, None]
+        vis = vis & (i < n) & (j < n)
+        # what stands behind a sequence is not looked at, NaN included
+        past = (torch.arange(N, device=q.device) >= n[:, 0])[:, None, :, None]
+        q, kf, vf = (x.masked_fill(past, 0) for x in (q, kf, vf))
+    z = (q.to(t) @ kf.transpose(2, 3).contiguous()) * scale
+    z = z.masked_fill(~vis[:, None], -math.inf)
+    top = z.detach().amax(3, keepdim=True)
+    e = torch.exp(z - torch.where(top == -math.inf, torch.zeros_like(top),
+                                  top))
+    total = e.sum(3, keepdim=True)
+    p = e / torch.where(total == 0, torch.ones_like(total), total)
+    return (p @ vf).to(q.dtype)
+
+
+def _rows16(t):
+    """t as the kernels read it: unit d stride, rows that start at 16 bytes."""
+    if (t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3])
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _WindowSDPA(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, lengths, scale):
+        q, k, v = (_rows16(t) for t in (q, k, v))
+        B, H, N, D = q.shape
+        # heads stand behind rows: what follows is a projection of all heads
+        o = torch.empty(B, N, H, D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device)
+        o = o.transpose(1, 2)
+        _EXT.wa_fwd(q, k, v, o, lse, lengths, window, sinks, scale)
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.cfg = (window, sinks, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        window, sinks, scale = ctx.cfg
+        B, H, N, D = q.shape
+        KV = k.shape[1]
+        dq = torch.empty(B, N, H, D, dtype=q.dtype,
+                         device=q.device).transpose(1, 2)
+        dk, dv = (torch.empty(B, N, KV, D, dtype=q.dtype,
+                              device=q.device).transpose(1, 2)
+                  for _ in range(2))
+        delta = torch.empty_like(lse)
+        part = torch.empty(_EXT.wa_part_floats(B, KV, N, D, window, sinks),
+                           dtype=torch.float32, device=q.device)
+        _EXT.wa_bwd(q, k, v, o, _rows16(dout), lse, delta, dq, dk, dv, part,
+                    lengths, window, sinks, scale)
+        return dq, dk, dv, None, None, None, None
+
+
+def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):
+    """Causal attention in which row i sees key j <= i if ``i - j < window`` or
+    ``j < sinks`` (the first tokens stay visible).
+
+    q: [B, H, N, D]; k, v: [B, KV, N, D] with H a multiple of KV (each key head
+    serves H/KV neighbouring query heads).  ``lengths``: optional int32 [B] on
+    the same device; rows and keys from a sequence's length on do not exist:
+    they may hold anything, their outputs and gradients are zero.  ``scale``:
+    positive, 1/sqrt(D) by default.  Returns [B, H, N, D], stored with the
+    heads behind the rows.
+
+    GPU, bf16, D 64 or 128: MFMA kernels forward and backward
+    (ops/csrc/window_attn_kernels.hip), reading any strides with unit d stride
+    and 16-byte rows.  Anything else: plain torch with the whole score matrix.
+    Values inside the lengths must be finite: a product with a weight of zero
+    lets a NaN or infinity reach rows that do not see it.
+    """
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("q must be [B, H, N, D], k and v [B, KV, N, D]")
+    B, H, N, D = q.shape
+    if k.shape[0] != B or k.shape[2] != N or k.shape[3] != D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ "
+                         "in B, N or D")
+    if k.shape[1] < 1 or H % k.shape[1]:
+        raise ValueError(f"{H} query heads do not divide over {k.shape[1]} "
+                         "key heads")
+    if not (q.dtype == k.dtype == v.dtype and q.is_floating_point()):
+        raise ValueError("q, k and v must have one floating type")
+    if not (q.device == k.device == v.device):
+        raise ValueError("q, k and v must be on one device")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be 1 or more, sinks 0 or more")
+    if lengths is not None and (lengths.dtype != torch.int32
+                                or tuple(lengths.shape) != (B,)
+                                or lengths.device != q.device):
+        raise ValueError(f"lengths must be int32 [{B}] on q's device")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
+    if (_require_ext(q) and q.dtype == torch.bfloat16 and D in (64, 128)
+            and q.numel()):
+        if lengths is not None:
+            lengths = lengths.contiguous()
+        return _WindowSDPA.apply(q, k, v, window, sinks, lengths, scale)
+    return _window_plain(q, k, v, window, sinks, lengths, scale)

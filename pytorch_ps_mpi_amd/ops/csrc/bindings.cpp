@@ -35,6 +35,18 @@ int ps_join_bwd(void* stream, void* const* t, float* const* stats,
                 void* const* sums, float* part, int bf16, int64_t groups,
                 int64_t rows, int64_t D, int layer, int gate_kind,
                 int64_t gate_step, float scale);
+int64_t ps_wa_part_floats(int64_t B, int64_t KV, int64_t N, int64_t D,
+                          int64_t window, int64_t sinks);
+int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
+              void* o, float* lse, const int32_t* lengths, const int64_t* st,
+              int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
+              int64_t window, int64_t sinks, float scale);
+int ps_wa_bwd(void* stream, const void* q, const void* k, const void* v,
+              const void* o, const void* go, float* lse, float* delta,
+              void* dq, void* dk, void* dv, float* part,
+              const int32_t* lengths, const int64_t* st, int64_t B, int64_t H,
+              int64_t KV, int64_t N, int64_t D, int64_t window, int64_t sinks,
+              float scale);
 int ps_reduce_accum(void* stream, float* dst, const void** srcs, int nsrc,
                     int src_is_bf16, int64_t n, float scale, float beta);
 int ps_f32_to_bf16(void* stream, const float* src, void* dst, int64_t n);
@@ -828,12 +840,115 @@ void fa_selfcheck(at::Tensor a, at::Tensor b, at::Tensor c) {
            "fa_selfcheck");
 }
 
+// ---- attention with a sliding window and visible first tokens -------------
+
+static void wa_rows(const at::Tensor& t, const char* name, const at::Tensor& q,
+                    int64_t heads, int64_t* st) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4,
+              name, " must be 4-D bf16 on GPU");
+  check_same_device(q, t, name);
+  TORCH_CHECK(t.size(0) == q.size(0) && t.size(1) == heads &&
+                  t.size(2) == q.size(2) && t.size(3) == q.size(3),
+              name, " has the wrong shape");
+  TORCH_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 &&
+                  t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+                  (uintptr_t)t.data_ptr() % 16 == 0,
+              name, " rows must be 16B-aligned with unit d-stride");
+  for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
+}
+
+// [B, heads, N, D] stored as [B, N, heads, D]
+static void wa_out(const at::Tensor& t, const char* name, const at::Tensor& q,
+                   int64_t heads) {
+  int64_t st[3];
+  wa_rows(t, name, q, heads, st);
+  TORCH_CHECK(t.transpose(1, 2).is_contiguous(), name,
+              " must be stored with heads behind rows");
+}
+
+static const int32_t* wa_lengths(const c10::optional<at::Tensor>& l,
+                                 const at::Tensor& q) {
+  if (!l.has_value()) return nullptr;
+  check_flat(*l, at::kInt, "lengths");
+  check_same_device(q, *l, "lengths");
+  TORCH_CHECK(l->numel() == q.size(0), "one length for each sequence");
+  return l->data_ptr<int32_t>();
+}
+
+static void wa_stat(const at::Tensor& t, const at::Tensor& q) {
+  check_flat(t, at::kFloat, "row statistics");
+  check_same_device(q, t, "row statistics");
+  TORCH_CHECK(t.numel() == q.size(0) * q.size(1) * q.size(2),
+              "row statistics size");
+}
+
+void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
+            at::Tensor lse, c10::optional<at::Tensor> lengths, int64_t window,
+            int64_t sinks, double scale) {
+  int64_t st[15] = {0};
+  TORCH_CHECK(k.dim() == 4 && q.dim() == 4, "q, k must be 4-D");
+  wa_rows(q, "q", q, q.size(1), st);
+  wa_rows(k, "k", q, k.size(1), st + 3);
+  wa_rows(v, "v", q, k.size(1), st + 6);
+  wa_out(o, "o", q, q.size(1));
+  wa_stat(lse, q);
+  const int32_t* len = wa_lengths(lengths, q);
+  const c10::DeviceGuard guard(q.device());
+  throw_on(ps_wa_fwd(cur_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     o.data_ptr(), lse.data_ptr<float>(), len, st, q.size(0),
+                     q.size(1), k.size(1), q.size(2), q.size(3), window, sinks,
+                     (float)scale),
+           "wa_fwd");
+}
+
+int64_t wa_part_floats(int64_t B, int64_t KV, int64_t N, int64_t D,
+                       int64_t window, int64_t sinks) {
+  return ps_wa_part_floats(B, KV, N, D, window, sinks);
+}
+
+void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
+            at::Tensor go, at::Tensor lse, at::Tensor delta, at::Tensor dq,
+            at::Tensor dk, at::Tensor dv, at::Tensor part,
+            c10::optional<at::Tensor> lengths, int64_t window, int64_t sinks,
+            double scale) {
+  int64_t st[15];
+  TORCH_CHECK(k.dim() == 4 && q.dim() == 4, "q, k must be 4-D");
+  wa_rows(q, "q", q, q.size(1), st);
+  wa_rows(k, "k", q, k.size(1), st + 3);
+  wa_rows(v, "v", q, k.size(1), st + 6);
+  wa_rows(o, "o", q, q.size(1), st + 9);
+  wa_rows(go, "dout", q, q.size(1), st + 12);
+  wa_out(dq, "dq", q, q.size(1));
+  wa_out(dk, "dk", q, k.size(1));
+  wa_out(dv, "dv", q, k.size(1));
+  wa_stat(lse, q);
+  wa_stat(delta, q);
+  check_flat(part, at::kFloat, "part");
+  check_same_device(q, part, "part");
+  TORCH_CHECK(part.numel() >= ps_wa_part_floats(q.size(0), k.size(1),
+                                                q.size(2), q.size(3), window,
+                                                sinks),
+              "part too small");
+  const int32_t* len = wa_lengths(lengths, q);
+  const c10::DeviceGuard guard(q.device());
+  throw_on(ps_wa_bwd(cur_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     o.data_ptr(), go.data_ptr(), lse.data_ptr<float>(),
+                     delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                     dv.data_ptr(), part.data_ptr<float>(), len, st, q.size(0),
+                     q.size(1), k.size(1), q.size(2), q.size(3), window, sinks,
+                     (float)scale),
+           "wa_bwd");
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
   m.def("fa_fwd", &fa_fwd, "MFMA-tiled flash attention forward");
   m.def("fa_bwd", &fa_bwd, "MFMA-tiled flash attention backward");
   m.def("fa_selfcheck", &fa_selfcheck, "16x16x32 MFMA fragment-layout check");
+  m.def("wa_fwd", &wa_fwd, "causal attention, sliding window and sinks");
+  m.def("wa_bwd", &wa_bwd);
+  m.def("wa_part_floats", &wa_part_floats);
   m.def("topk_encode_thresh", &topk_encode_thresh,
         "variable-k magnitude-threshold select (k_used -> device header)");
   m.def("colsum", &colsum, "column sum (bias grads)");

@@ -1,0 +1,701 @@
+// window_attn_kernels.hip — causal attention with a sliding window and first
+// tokens that stay visible, forward and backward (gfx950 / MI355X).
+//
+//   vis(i, j) = j <= i and (i - j < window or j < sinks), i, j < length
+//   P = softmax over vis of scale * q.k ;  o = P v ;  rows past the length: 0
+//   dV = P^T dO ; dP = dO V^T ; dS = P * (dP - rowsum(dO * O)) ;
+//   dQ = scale * dS K ; dK = scale * dS^T Q
+//
+// q, k, v: bf16 of any strides with unit d stride, heads in groups that share
+// keys and values.  D is 64 or 128.  Scores, statistics and sums in fp32, P and
+// dS rounded to bf16 as operands of the matrix instructions.
+//
+// Layout.  mfma 32x32x16: operand rows (or columns) are lane % 32, its
+// contraction index 8 * (lane / 32) + j; the result's column is lane % 32, its
+// row 8 * (r / 4) + 4 * (lane / 32) + r % 4 for register r.  Scores are computed
+// transposed to what owns them: a wave that owns 32 queries holds them as
+// columns (S^T = K Q^T), one that owns 32 keys holds those as columns
+// (S = Q K^T).  So statistics of a row are per-lane numbers (forward, dQ), and
+// a result's registers 8s..8s+7 are, as they are, the operand of the next
+// product for the contraction rows 16s + {0..3, 8..11} + 4 * (lane / 32): the
+// other operand is read from LDS in that same order, by the transposing read.
+// P and dS never go through LDS.
+//
+// Tiles of 64 rows stand in LDS row-major with their 16-byte granules swizzled
+// (wa_swz) so that neither the row reads nor the transposing reads meet in a
+// bank.  Tiles are double-buffered: the next one travels to registers while
+// this one is worked on; one barrier a tile.
+//
+// Four waves share a tile.  In the forward and dQ kernels they are up to four
+// heads of a group (same rows, same keys) times neighbouring rows; in the dK/dV
+// kernel four neighbouring strips of 32 keys, and the block walks all heads of
+// the group, so that shared heads are summed in registers, without atomics.
+//
+// The first tokens are seen by all rows: their dK/dV would be one block's work
+// of N rows among blocks of `window` rows.  Rows behind the window are split
+// over further blocks whose parts a last kernel adds in fixed order.
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <cstdint>
+
+typedef __attribute__((ext_vector_type(8))) __bf16 wa_bf8;
+typedef __attribute__((ext_vector_type(2))) __bf16 wa_bf2;
+typedef __attribute__((ext_vector_type(2))) float wa_f2;
+typedef __attribute__((ext_vector_type(4))) short wa_s4;
+typedef __attribute__((ext_vector_type(8))) short wa_s8;
+typedef __attribute__((ext_vector_type(16))) float wa_f16;
+typedef __attribute__((ext_vector_type(4))) uint32_t wa_u4;
+typedef __attribute__((address_space(3))) wa_s4 wa_lds_s4;
+
+#define WA_BLOCK 256
+#define WA_T 64           // rows of a tile
+#define WA_KB 128         // keys of a dK/dV block
+#define WA_LOG2E 1.4426950408889634f
+
+struct WaTensor {
+  const __bf16* p;
+  int64_t sB, sH, sN;
+};
+
+struct WaArgs {
+  WaTensor q, k, v, o, go;
+  __bf16 *out, *dq, *dk, *dv;   // out, dq: [B,N,H,D]; dk, dv: [B,N,KV,D]
+  float *lse, *delta;           // [B,H,N]; lse of base 2
+  float* part;                  // dK, dV parts of the first tokens
+  const int32_t* lengths;       // [B], or null
+  int B, H, KV, N, window, sinks;
+  int chunks, sinkrows;         // parts of each sink block, rows it holds
+  float scale;
+};
+
+template <int D>
+__device__ __forceinline__ int wa_swz(int row) {
+  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                  : ((row & 2) << 1) | ((row >> 2) & 3);
+}
+
+__device__ __forceinline__ wa_f16 wa_mfma(wa_bf8 a, wa_bf8 b, wa_f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float wa_exp2(float x) {
+  return __builtin_amdgcn_exp2f(x);
+}
+
+// the other half wave's value joined to one's own
+__device__ __forceinline__ float wa_other_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float wa_other_sum(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ uint32_t wa_pack(float a, float b) {
+  const wa_bf2 v = __builtin_convertvector((wa_f2){a, b}, wa_bf2);
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// registers 8s..8s+7 of a result as an operand
+__device__ __forceinline__ wa_bf8 wa_operand(const wa_f16& f, int s) {
+  wa_u4 u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] = wa_pack(f[8 * s + 2 * j], f[8 * s + 2 * j + 1]);
+  return __builtin_bit_cast(wa_bf8, u);
+}
+
+// Operands of 16 columns of D for a row of the tensor, straight from memory.
+template <int D>
+__device__ __forceinline__ void wa_row(const __bf16* row, int half, wa_bf8* f) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) f[kk] = *(const wa_bf8*)(row + kk * 16 + half * 8);
+}
+
+// A tile on its way: 64 rows of D elements by 256 threads.  Rows past the
+// length take the last one's place: what stands there is never read.
+template <int D>
+struct WaStage {
+  static constexpr int G = D / 8, STEP = WA_BLOCK / G, CNT = WA_T / STEP;
+  wa_u4 v[CNT];
+  __device__ __forceinline__ void load(const __bf16* base, int64_t sN, int row0, int len) {
+    const int g = threadIdx.x % G, r = threadIdx.x / G;
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int row = min(row0 + r + i * STEP, len - 1);
+      v[i] = *(const wa_u4*)(base + row * sN + g * 8);
+    }
+  }
+  __device__ __forceinline__ void store(__bf16* lds) const {
+    const int g = threadIdx.x % G, r = threadIdx.x / G;
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int row = r + i * STEP;
+      *(wa_u4*)(lds + row * D + ((g ^ wa_swz<D>(row)) * 8)) = v[i];
+    }
+  }
+};
+
+// Row operand: rows sub*32 + lane%32 of a tile, columns 16kk + 8*half ...
+template <int D>
+struct WaRows {
+  int base, swz, half;
+  __device__ __forceinline__ WaRows(int lane) {
+    base = (lane & 31) * D;
+    swz = wa_swz<D>(lane & 31);
+    half = lane >> 5;
+  }
+  __device__ __forceinline__ wa_bf8 get(const __bf16* tile, int sub, int kk) const {
+    return *(const wa_bf8*)(tile + sub * 32 * D + base + (((2 * kk + half) ^ swz) * 8));
+  }
+};
+
+// Transposed operand: row is column 32dt + lane%32 of the tile, contraction
+// over the tile's rows 16ks + {0..3, 8..11} + 4*half.
+template <int D>
+struct WaCols {
+  int at[2][D / 32];
+  __device__ __forceinline__ WaCols(int lane) {
+    const int i = lane & 15, grp = lane >> 4, half = grp >> 1;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const int row = 8 * jj + 4 * half + (i >> 2);
+        const int col = 32 * dt + 16 * (grp & 1) + (i & 3) * 4;
+        at[jj][dt] = row * D + ((col >> 3) ^ wa_swz<D>(row)) * 8 + (col & 7);
+      }
+  }
+  __device__ __forceinline__ wa_bf8 get(const __bf16* tile, int ks, int dt) const {
+    const wa_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (wa_lds_s4*)(tile + ks * 16 * D + at[0][dt]));
+    const wa_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (wa_lds_s4*)(tile + ks * 16 * D + at[1][dt]));
+    const wa_s8 s = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(wa_bf8, s);
+  }
+};
+
+// Stores a transposed result (columns: 32 rows of the tensor, rows: D) times f,
+// 16 bytes a lane: the half waves swap so that each holds 8 neighbours.
+template <int D>
+__device__ __forceinline__ void wa_store(__bf16* row, const wa_f16* acc, float f,
+                                         int half, bool write) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        u[j] = wa_pack(acc[dt][8 * p + 2 * j] * f, acc[dt][8 * p + 2 * j + 1] * f);
+      auto a = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false);
+      auto b = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
+      const wa_u4 w = {a[0], b[0], a[1], b[1]};
+      if (write) *(wa_u4*)(row + 32 * dt + 16 * p + 8 * half) = w;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// where a block of the forward and dQ kernels works, and its tiles
+// ---------------------------------------------------------------------------
+
+struct WaPlace {
+  int b, kv, head, row0, last, len;  // rows row0 .. last of this block
+  int wrow;                          // this wave's first row
+  int nsink, first, count;           // tiles: nsink from 0, the rest from first
+  __device__ __forceinline__ int tile(int it) const {
+    return it < nsink ? it : first + it - nsink;
+  }
+};
+
+__device__ __forceinline__ int wa_len(const WaArgs& a, int b) {
+  return a.lengths ? max(0, min(a.lengths[b], a.N)) : a.N;
+}
+
+__device__ __forceinline__ WaPlace wa_place(const WaArgs& a, int gw) {
+  WaPlace w;
+  const int rw = 4 / gw, rows = 32 * rw, wave = threadIdx.x >> 6;
+  const int blocks = (a.N + rows - 1) / rows, hb = a.H / gw;
+  const int u = blockIdx.x / blocks;
+  // last rows first: in a short sequence they have the most keys
+  const int blk = blocks - 1 - (blockIdx.x - u * blocks);
+  w.b = u / hb;
+  const int h0 = (u - w.b * hb) * gw;
+  w.head = h0 + wave % gw;
+  w.kv = h0 / (a.H / a.KV);
+  w.len = wa_len(a, w.b);
+  w.row0 = blk * rows;
+  w.last = min(w.row0 + rows, w.len) - 1;
+  w.wrow = w.row0 + (wave / gw) * 32;
+  w.first = max(0, w.row0 - a.window + 1) / WA_T;
+  w.nsink = min((a.sinks + WA_T - 1) / WA_T, w.first);
+  w.count = w.last < w.row0 ? 0 : w.nsink + w.last / WA_T + 1 - w.first;
+  return w;
+}
+
+// Of rows r0..r0+31 and keys k0..k0+n-1: 0 none visible, 1 some, 2 all
+__device__ __forceinline__ int wa_seen(const WaArgs& a, int r0, int k0, int n) {
+  if (k0 > r0 + 31) return 0;
+  if (k0 >= a.sinks && r0 - (k0 + n - 1) >= a.window) return 0;
+  if (k0 + n - 1 <= r0 && (r0 + 31 - k0 < a.window || k0 + n <= a.sinks)) return 2;
+  return 1;
+}
+
+__device__ __forceinline__ bool wa_vis(const WaArgs& a, int i, int j) {
+  return j <= i && (i - j < a.window || j < a.sinks);
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+
+template <int D>
+__global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const WaPlace w = wa_place(a, gw);
+  const int row = w.wrow + col;
+  __bf16* out = a.out + (((int64_t)w.b * a.N + row) * a.H + w.head) * D;
+  wa_f16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = (wa_f16)(0.0f);
+  if (w.count == 0) {  // rows past the length
+    wa_store<D>(out, acc, 0.0f, half, row < a.N);
+    return;
+  }
+  const __bf16* kb = a.k.p + w.b * a.k.sB + w.kv * a.k.sH;
+  const __bf16* vb = a.v.p + w.b * a.v.sB + w.kv * a.v.sH;
+  wa_bf8 qf[D / 16];
+  wa_row<D>(a.q.p + w.b * a.q.sB + w.head * a.q.sH + min(row, w.len - 1) * a.q.sN, half, qf);
+  const WaRows<D> rows(lane);
+  const WaCols<D> cols(lane);
+  WaStage<D> sk, sv;
+  sk.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
+  sv.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+  const float c = a.scale * WA_LOG2E;
+  float m = -3.0e38f, l = 0.0f;  // l: this half wave's keys
+  for (int it = 0; it < w.count; ++it) {
+    __bf16* tk = lds[it & 1][0];
+    __bf16* tv = lds[it & 1][1];
+    const int k0 = w.tile(it) * WA_T;
+    sk.store(tk);
+    sv.store(tv);
+    if (it + 1 < w.count) {
+      sk.load(kb, a.k.sN, w.tile(it + 1) * WA_T, w.len);
+      sv.load(vb, a.v.sN, w.tile(it + 1) * WA_T, w.len);
+    }
+    __syncthreads();
+    const int seen = wa_seen(a, w.wrow, k0, WA_T);
+    if (seen == 0) continue;
+    wa_f16 s[2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      s[sub] = (wa_f16)(0.0f);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        s[sub] = wa_mfma(rows.get(tk, sub, kk), qf[kk], s[sub]);
+    }
+    if (seen == 1) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + sub * 32 + 8 * (r / 4) + 4 * half + r % 4;
+          if (!wa_vis(a, row, key)) s[sub][r] = -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+    const float mn = fmaxf(m, wa_other_max(top) * c);
+    if (__any(mn > m)) {
+      const float f = wa_exp2(m - mn);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) acc[t] *= f;
+      m = mn;
+    }
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[sub][r] = wa_exp2(fmaf(s[sub][r], c, -m));
+        l += s[sub][r];
+      }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const wa_bf8 p = wa_operand(s[ks >> 1], ks & 1);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) acc[t] = wa_mfma(cols.get(tv, ks, t), p, acc[t]);
+    }
+  }
+  l = wa_other_sum(l);
+  const bool in = row < w.len;
+  wa_store<D>(out, acc, 1.0f / l, half, in);
+  if (in) {
+    if (half == 0) a.lse[((int64_t)w.b * a.H + w.head) * a.N + row] = m + __builtin_amdgcn_logf(l);
+  } else if (row < a.N) {
+    for (int e = half * 8; e < D; e += 16) *(wa_u4*)(out + e) = (wa_u4)(0u);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward: dQ, and rowsum(dO * O) for the next kernel
+// ---------------------------------------------------------------------------
+
+template <int D>
+__global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const WaPlace w = wa_place(a, gw);
+  const int row = w.wrow + col;
+  __bf16* out = a.dq + (((int64_t)w.b * a.N + row) * a.H + w.head) * D;
+  wa_f16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = (wa_f16)(0.0f);
+  if (w.count == 0) {
+    wa_store<D>(out, acc, 0.0f, half, row < a.N);
+    return;
+  }
+  const __bf16* kb = a.k.p + w.b * a.k.sB + w.kv * a.k.sH;
+  const __bf16* vb = a.v.p + w.b * a.v.sB + w.kv * a.v.sH;
+  const bool in = row < w.len;
+  const int at = min(row, w.len - 1);
+  wa_bf8 qf[D / 16], gf[D / 16];
+  wa_row<D>(a.q.p + w.b * a.q.sB + w.head * a.q.sH + at * a.q.sN, half, qf);
+  wa_row<D>(a.go.p + w.b * a.go.sB + w.head * a.go.sH + at * a.go.sN, half, gf);
+  float delta = 0.0f;
+  {
+    const __bf16* orow = a.o.p + w.b * a.o.sB + w.head * a.o.sH + at * a.o.sN;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const wa_bf8 of = *(const wa_bf8*)(orow + kk * 16 + half * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf((float)of[j], (float)gf[kk][j], delta);
+    }
+    delta = wa_other_sum(delta);
+  }
+  const int64_t stat = ((int64_t)w.b * a.H + w.head) * a.N + at;
+  const float lse = a.lse[stat];
+  if (in && half == 0) a.delta[stat] = delta;
+  const WaRows<D> rows(lane);
+  const WaCols<D> cols(lane);
+  WaStage<D> sk, sv;
+  sk.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
+  sv.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+  const float c = a.scale * WA_LOG2E;
+  for (int it = 0; it < w.count; ++it) {
+    __bf16* tk = lds[it & 1][0];
+    __bf16* tv = lds[it & 1][1];
+    const int k0 = w.tile(it) * WA_T;
+    sk.store(tk);
+    sv.store(tv);
+    if (it + 1 < w.count) {
+      sk.load(kb, a.k.sN, w.tile(it + 1) * WA_T, w.len);
+      sv.load(vb, a.v.sN, w.tile(it + 1) * WA_T, w.len);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const int seen = wa_seen(a, w.wrow, k0 + sub * 32, 32);
+      if (seen == 0) continue;
+      wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        s = wa_mfma(rows.get(tk, sub, kk), qf[kk], s);
+        p = wa_mfma(rows.get(tv, sub, kk), gf[kk], p);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float e = wa_exp2(fmaf(s[r], c, -lse));
+        if (seen == 1 &&
+            !wa_vis(a, row, k0 + sub * 32 + 8 * (r / 4) + 4 * half + r % 4))
+          e = 0.0f;
+        s[r] = e * (p[r] - delta);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const wa_bf8 d = wa_operand(s, ks);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+          acc[t] = wa_mfma(cols.get(tk, sub * 2 + ks, t), d, acc[t]);
+      }
+    }
+  }
+  wa_store<D>(out, acc, a.scale, half, in);
+  if (!in && row < a.N)
+    for (int e = half * 8; e < D; e += 16) *(wa_u4*)(out + e) = (wa_u4)(0u);
+}
+
+// ---------------------------------------------------------------------------
+// backward: dK and dV
+// ---------------------------------------------------------------------------
+// Block (u, x): u = sequence and key head; x < key blocks: 128 keys and the
+// rows that see them by the window.  x beyond: a part of the rows behind the
+// window of a block of first tokens.
+
+template <int D>
+__global__ void __launch_bounds__(WA_BLOCK, 1) k_wa_dkv(const WaArgs a) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][WA_T];
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int wave = threadIdx.x >> 6;
+  const int nkb = (a.N + WA_KB - 1) / WA_KB;
+  const int nsb = a.chunks ? (a.sinks + WA_KB - 1) / WA_KB : 0;
+  const int per = nkb + nsb * a.chunks;
+  const int u = blockIdx.x / per, x = blockIdx.x - u * per;
+  const int b = u / a.KV, kv = u - b * a.KV, G = a.H / a.KV;
+  const int len = wa_len(a, b);
+  // the rows, in tiles, of each head
+  const bool behind = x >= nkb;
+  const int kblk = behind ? (x - nkb) / a.chunks : x;
+  const int chunk = behind ? (x - nkb) % a.chunks : 0;
+  const int k0 = kblk * WA_KB;
+  // behind here the window sees none of this block's keys
+  const int64_t wend = (int64_t)k0 + WA_KB - 1 + a.window;
+  const int tw = (int)((min(wend, (int64_t)len) + WA_T - 1) / WA_T);
+  const int tn = (len + WA_T - 1) / WA_T;
+  const bool sinkblk = k0 < a.sinks;
+  int t0, total;  // first tile, tiles of a head
+  if (!behind) {
+    t0 = k0 / WA_T;
+    total = (sinkblk && a.chunks == 0 ? tn : tw) - t0;
+  } else {
+    t0 = tw;
+    total = tn - tw;
+  }
+  total = max(total, 0);
+  int it0 = 0, it1 = total * G;  // (head, tile) pairs
+  if (behind) {
+    const int each = (it1 + a.chunks - 1) / a.chunks;
+    it0 = min(chunk * each, it1);
+    it1 = min(it0 + each, it1);
+  }
+  const int wk = k0 + wave * 32;   // this wave's first key
+  const int key = wk + col;
+  wa_f16 ak[D / 32], av[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = (wa_f16)(0.0f);
+  if (it0 < it1 && k0 < len) {
+    wa_bf8 kf[D / 16], vf[D / 16];
+    const int at = min(key, len - 1);
+    wa_row<D>(a.k.p + b * a.k.sB + kv * a.k.sH + at * a.k.sN, half, kf);
+    wa_row<D>(a.v.p + b * a.v.sB + kv * a.v.sH + at * a.v.sN, half, vf);
+    const WaRows<D> rows(lane);
+    const WaCols<D> cols(lane);
+    WaStage<D> sq, sg;
+    float sl = 0.0f, sd = 0.0f;
+    const float c = a.scale * WA_LOG2E;
+    auto load = [&](int it) {
+      const int head = kv * G + it / total, r0 = (t0 + it % total) * WA_T;
+      sq.load(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN, r0, len);
+      sg.load(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN, r0, len);
+      if (threadIdx.x < WA_T) {
+        const int r = r0 + threadIdx.x;
+        const int64_t i = ((int64_t)b * a.H + head) * a.N + min(r, len - 1);
+        sl = r < len ? a.lse[i] : INFINITY;  // no weight for rows that are not
+        sd = a.delta[i];
+      }
+    };
+    load(it0);
+    for (int it = it0; it < it1; ++it) {
+      const int buf = (it - it0) & 1;
+      __bf16* tq = lds[buf][0];
+      __bf16* tg = lds[buf][1];
+      sq.store(tq);
+      sg.store(tg);
+      if (threadIdx.x < WA_T) {
+        stat[buf][0][threadIdx.x] = sl;
+        stat[buf][1][threadIdx.x] = sd;
+      }
+      const int r0 = (t0 + it % total) * WA_T;
+      if (it + 1 < it1) load(it + 1);
+      __syncthreads();
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int rs = r0 + sub * 32;
+        const int seen = wa_seen(a, rs, wk, 32);
+        if (seen == 0) continue;
+        wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          s = wa_mfma(rows.get(tq, sub, kk), kf[kk], s);
+          p = wa_mfma(rows.get(tg, sub, kk), vf[kk], p);
+        }
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int r = sub * 32 + 8 * r4 + 4 * half;
+          const float4 ls = *(const float4*)&stat[buf][0][r];
+          const float4 de = *(const float4*)&stat[buf][1][r];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float lj = j == 0 ? ls.x : j == 1 ? ls.y : j == 2 ? ls.z : ls.w;
+            const float dj = j == 0 ? de.x : j == 1 ? de.y : j == 2 ? de.z : de.w;
+            float e = wa_exp2(fmaf(s[4 * r4 + j], c, -lj));
+            if (seen == 1 && !wa_vis(a, r0 + r + j, key)) e = 0.0f;
+            s[4 * r4 + j] = e;
+            p[4 * r4 + j] = e * (p[4 * r4 + j] - dj);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const wa_bf8 pf = wa_operand(s, ks), df = wa_operand(p, ks);
+#pragma unroll
+          for (int t = 0; t < D / 32; ++t) {
+            av[t] = wa_mfma(cols.get(tg, sub * 2 + ks, t), pf, av[t]);
+            ak[t] = wa_mfma(cols.get(tq, sub * 2 + ks, t), df, ak[t]);
+          }
+        }
+      }
+    }
+  }
+  if (sinkblk && a.chunks) {
+    // fp32 parts [u][key block][1 + chunks][dK, dV][sinkrows][D]
+    const int slot = behind ? 1 + chunk : 0;
+    const int mine = min(a.sinks - k0, WA_KB);  // rows of first tokens here
+    float* p = a.part + ((((int64_t)u * nsb + kblk) * (1 + a.chunks) + slot) * 2
+                         * a.sinkrows + wave * 32 + col) * D;
+    if (wave * 32 + col < mine) {
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int d = 32 * t + 8 * r4 + 4 * half;
+          const float4 k4 = {ak[t][4 * r4], ak[t][4 * r4 + 1], ak[t][4 * r4 + 2], ak[t][4 * r4 + 3]};
+          const float4 v4 = {av[t][4 * r4], av[t][4 * r4 + 1], av[t][4 * r4 + 2], av[t][4 * r4 + 3]};
+          *(float4*)(p + d) = k4;
+          *(float4*)(p + (int64_t)a.sinkrows * D + d) = v4;
+        }
+    }
+    if (behind) return;
+  }
+  const bool write = key < a.N && !(sinkblk && a.chunks && key < a.sinks);
+  const int64_t off = (((int64_t)b * a.N + key) * a.KV + kv) * D;
+  wa_store<D>(a.dk + off, ak, a.scale, half, write);
+  wa_store<D>(a.dv + off, av, 1.0f, half, write);
+}
+
+// dK and dV of the first tokens: the parts in order.
+template <int D>
+__global__ void __launch_bounds__(D) k_wa_sink_sum(const WaArgs a) {
+  const int key = blockIdx.x, u = blockIdx.y;
+  const int b = u / a.KV, kv = u - b * a.KV, d = threadIdx.x;
+  const int nsb = (a.sinks + WA_KB - 1) / WA_KB, kblk = key / WA_KB;
+  const float* p = a.part + (((int64_t)u * nsb + kblk) * (1 + a.chunks) * 2 * a.sinkrows
+                             + key % WA_KB) * D + d;
+  float sk = 0.0f, sv = 0.0f;
+  for (int s = 0; s <= a.chunks; ++s) {
+    sk += p[(int64_t)s * 2 * a.sinkrows * D];
+    sv += p[((int64_t)s * 2 + 1) * a.sinkrows * D];
+  }
+  const int64_t off = (((int64_t)b * a.N + key) * a.KV + kv) * D + d;
+  a.dk[off] = (__bf16)(sk * a.scale);
+  a.dv[off] = (__bf16)sv;
+}
+
+// ---------------------------------------------------------------------------
+
+// How many blocks share the rows that see a block of first tokens from behind
+// its window: about the work of an ordinary block each.  0: no such rows.
+static int wa_chunks(int64_t N, int64_t window, int64_t sinks) {
+  if (sinks <= 0 || N <= window) return 0;
+  const int64_t rows = N - window;  // behind the first key's window
+  int64_t n = (rows + window + WA_KB - 1) / (window + WA_KB);
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+static int wa_sinkrows(int64_t sinks) {
+  return (int)(sinks < WA_KB ? sinks : WA_KB);
+}
+
+extern "C" int64_t ps_wa_part_floats(int64_t B, int64_t KV, int64_t N, int64_t D,
+                                     int64_t window, int64_t sinks) {
+  if (sinks > N) sinks = N;
+  const int64_t ch = wa_chunks(N, window, sinks);
+  if (ch == 0) return 0;
+  const int64_t nsb = (sinks + WA_KB - 1) / WA_KB;
+  return B * KV * nsb * (1 + ch) * 2 * wa_sinkrows(sinks) * D;
+}
+
+static int wa_fill(WaArgs& a, const int64_t* st, int64_t B, int64_t H, int64_t KV,
+                   int64_t N, int64_t window, int64_t sinks, float scale,
+                   const int32_t* lengths) {
+  if (N > (1 << 30) || B * H > 0x7fffffff || N < 1 || KV < 1 || H % KV || window < 1 ||
+      sinks < 0 || !(scale > 0.0f))
+    return 9003;
+  WaTensor* t[5] = {&a.q, &a.k, &a.v, &a.o, &a.go};
+  for (int i = 0; i < 5; ++i) {
+    t[i]->sB = st[3 * i]; t[i]->sH = st[3 * i + 1]; t[i]->sN = st[3 * i + 2];
+  }
+  a.B = (int)B; a.H = (int)H; a.KV = (int)KV; a.N = (int)N;
+  a.window = (int)(window < N ? window : N);
+  a.sinks = (int)(sinks < N ? sinks : N);
+  a.chunks = wa_chunks(N, a.window, a.sinks);
+  a.sinkrows = wa_sinkrows(a.sinks);
+  a.scale = scale;
+  a.lengths = lengths;
+  return 0;
+}
+
+static int wa_heads_a_block(int64_t G) { return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1; }
+
+static int64_t wa_row_grid(int64_t B, int64_t H, int64_t N, int gw) {
+  const int64_t rows = 128 / gw;
+  return B * (H / gw) * ((N + rows - 1) / rows);
+}
+
+// st: strides (B, H, N) of q, k, v, o, go; o is written as [B, N, H, D]
+extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
+                         void* o, float* lse, const int32_t* lengths,
+                         const int64_t* st, int64_t B, int64_t H, int64_t KV,
+                         int64_t N, int64_t D, int64_t window, int64_t sinks,
+                         float scale) {
+  if (B <= 0 || N <= 0) return 0;
+  WaArgs a{};
+  if (int e = wa_fill(a, st, B, H, KV, N, window, sinks, scale, lengths)) return e;
+  a.q.p = (const __bf16*)q; a.k.p = (const __bf16*)k; a.v.p = (const __bf16*)v;
+  a.out = (__bf16*)o; a.lse = lse;
+  const int gw = wa_heads_a_block(H / KV);
+  const int64_t grid = wa_row_grid(B, H, N, gw);
+  if (grid > 0x7fffffff || (D != 64 && D != 128)) return 9003;
+  hipStream_t s = (hipStream_t)stream;
+  if (D == 64) hipLaunchKernelGGL((k_wa_fwd<64>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
+  else hipLaunchKernelGGL((k_wa_fwd<128>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
+  return (int)hipGetLastError();
+}
+
+extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void* v,
+                         const void* o, const void* go, float* lse, float* delta,
+                         void* dq, void* dk, void* dv, float* part,
+                         const int32_t* lengths, const int64_t* st, int64_t B,
+                         int64_t H, int64_t KV, int64_t N, int64_t D,
+                         int64_t window, int64_t sinks, float scale) {
+  if (B <= 0 || N <= 0) return 0;
+  WaArgs a{};
+  if (int e = wa_fill(a, st, B, H, KV, N, window, sinks, scale, lengths)) return e;
+  a.q.p = (const __bf16*)q; a.k.p = (const __bf16*)k; a.v.p = (const __bf16*)v;
+  a.o.p = (const __bf16*)o; a.go.p = (const __bf16*)go;
+  a.lse = lse; a.delta = delta; a.part = part;
+  a.dq = (__bf16*)dq; a.dk = (__bf16*)dk; a.dv = (__bf16*)dv;
+  const int gw = wa_heads_a_block(H / KV);
+  const int64_t grid = wa_row_grid(B, H, N, gw);
+  const int64_t nsb = a.chunks ? (a.sinks + WA_KB - 1) / WA_KB : 0;
+  const int64_t kgrid = B * KV * ((N + WA_KB - 1) / WA_KB + nsb * a.chunks);
+  if (grid > 0x7fffffff || kgrid > 0x7fffffff || B * KV > 65535 ||
+      (D != 64 && D != 128))
+    return 9003;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 sums((unsigned)a.sinks, (unsigned)(B * KV));
+  if (D == 64) {
+    hipLaunchKernelGGL((k_wa_dq<64>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
+    hipLaunchKernelGGL((k_wa_dkv<64>), dim3((unsigned)kgrid), dim3(WA_BLOCK), 0, s, a);
+    if (a.chunks) hipLaunchKernelGGL((k_wa_sink_sum<64>), sums, dim3(64), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((k_wa_dq<128>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
+    hipLaunchKernelGGL((k_wa_dkv<128>), dim3((unsigned)kgrid), dim3(WA_BLOCK), 0, s, a);
+    if (a.chunks) hipLaunchKernelGGL((k_wa_sink_sum<128>), sums, dim3(128), 0, s, a);
+  }
+  return (int)hipGetLastError();
+}
