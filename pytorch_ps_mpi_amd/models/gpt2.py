@@ -8,42 +8,100 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.attn import fused_sdpa_qkv
+from ..ops.attn import fused_sdpa_qkv, fused_window_sdpa
 from ..ops.ce import fused_cross_entropy
 from ..ops.linear import FusedLinear
-from ..ops.ln import FusedLayerNorm
+from ..ops.ln import FusedLayerNorm, fused_gated_residual
+from ..ops.rope import AxialRotary
 
 
 class CausalBlock(nn.Module):
-    def __init__(self, dim, heads):
+    """One transformer block.
+
+    window, sinks : attention to the last ``window`` tokens and the first
+        ``sinks`` ones; kv_heads : key heads, each shared by heads/kv_heads
+        query heads; rotary : AxialRotary that turns q and k.  Any of them
+        takes the windowed kernels, none the full causal ones.
+    layer_scale : start value of a gate for each channel of both branches;
+        the norms then ride with gate and residual in one pass (``joined``).
+    """
+
+    def __init__(self, dim, heads, window=None, sinks=0, kv_heads=None,
+                 rotary=None, layer_scale=None):
         super().__init__()
         self.n1 = FusedLayerNorm(dim)
-        self.qkv = FusedLinear(dim, 3 * dim)
+        self.local = not (window is None and kv_heads is None
+                          and rotary is None)
+        self.window, self.sinks = window, sinks
+        self.kv_heads = kv_heads or heads
+        self.rotary = rotary
+        self.qkv = FusedLinear(
+            dim, dim // heads * (heads + 2 * self.kv_heads))
         self.proj = FusedLinear(dim, dim)
         self.n2 = FusedLayerNorm(dim)
         self.fc1 = FusedLinear(dim, 4 * dim)
         self.fc2 = FusedLinear(4 * dim, dim)
         self.heads = heads
+        if layer_scale is not None:
+            self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
+            self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
 
-    def forward(self, x):
-        B, T, D = x.shape
-        qkv = self.qkv(self.n1(x)).view(B, T, 3, self.heads, D // self.heads)
-        y = fused_sdpa_qkv(qkv, is_causal=True)  # [B, H, T, Dh]
-        y = y.transpose(1, 2).reshape(B, T, D)
-        x = x + self.proj(y)
-        x = x + self.fc2(F.gelu(self.fc1(self.n2(x))))
+    def attend(self, h, pos=None):
+        B, T, D = h.shape
+        hd = D // self.heads
+        if not self.local:
+            qkv = self.qkv(h).view(B, T, 3, self.heads, hd)
+            y = fused_sdpa_qkv(qkv, is_causal=True)  # [B, H, T, Dh]
+        else:
+            kv = self.kv_heads
+            q, k, v = self.qkv(h).view(B, T, -1, hd).split(
+                [self.heads, kv, kv], 2)
+            if self.rotary is not None:
+                q, k = self.rotary(q, k, pos)
+            y = fused_window_sdpa(q.transpose(1, 2), k.transpose(1, 2),
+                                  v.transpose(1, 2), self.window or T,
+                                  self.sinks)
+        return self.proj(y.transpose(1, 2).reshape(B, T, D))
+
+    def mlp(self, h):
+        return self.fc2(F.gelu(self.fc1(h)))
+
+    def forward(self, x, pos=None):
+        x = x + self.attend(self.n1(x), pos)
+        x = x + self.mlp(self.n2(x))
         return x
+
+    def joined(self, x, h, after, pos=None):
+        """x: residual stream, h: its norm n1.  Returns the stream behind this
+        block and its norm by ``after``."""
+        x, h = fused_gated_residual(x, self.attend(h, pos), self.n2.weight,
+                                    self.n2.bias, gate=self.g1,
+                                    eps=self.n2.eps)
+        return fused_gated_residual(x, self.mlp(h), after.weight, after.bias,
+                                    gate=self.g2, eps=after.eps)
 
 
 class GPT2(nn.Module):
-    def __init__(self, vocab=50257, ctx=1024, dim=768, depth=12, heads=12):
+    """window, sinks, kv_heads, layer_scale: see CausalBlock; rotary=True
+    takes rotary positions in place of learned ones."""
+
+    def __init__(self, vocab=50257, ctx=1024, dim=768, depth=12, heads=12,
+                 window=None, sinks=0, kv_heads=None, rotary=False,
+                 layer_scale=None):
         super().__init__()
+        if dim % heads or heads % (kv_heads or heads):
+            raise ValueError("heads must divide dim, kv_heads must divide "
+                             "heads")
         self.wte = nn.Embedding(vocab, dim)
-        self.wpe = nn.Embedding(ctx, dim)
-        self.blocks = nn.ModuleList(CausalBlock(dim, heads)
-                                    for _ in range(depth))
+        rot = AxialRotary(dim // heads, (dim // heads // 2,)) if rotary \
+            else None
+        self.wpe = None if rotary else nn.Embedding(ctx, dim)
+        self.blocks = nn.ModuleList(
+            CausalBlock(dim, heads, window, sinks, kv_heads, rot, layer_scale)
+            for _ in range(depth))
         self.norm = FusedLayerNorm(dim)
         self.ctx = ctx
+        self.layer_scale = layer_scale
         for m in self.modules():
             if isinstance(m, nn.Linear):
                 nn.init.normal_(m.weight, std=0.02)
@@ -55,10 +113,20 @@ class GPT2(nn.Module):
     def forward(self, idx):
         B, T = idx.shape
         pos = torch.arange(T, device=idx.device)
-        x = self.wte(idx) + self.wpe(pos)[None]
-        for blk in self.blocks:
-            x = blk(x)
-        x = self.norm(x)
+        x = self.wte(idx)
+        if self.wpe is not None:
+            x = x + self.wpe(pos)[None]
+        pos = pos[None]  # one axis
+        if self.layer_scale is None:
+            for blk in self.blocks:
+                x = blk(x, pos)
+            x = self.norm(x)
+        else:
+            norms = [blk.n1 for blk in self.blocks] + [self.norm]
+            h = norms[0](x)
+            for blk, after in zip(self.blocks, norms[1:]):
+                x, h = blk.joined(x, h, after, pos)
+            x = h
         # tied output head
         return x @ self.wte.weight.t()
 
@@ -72,6 +140,6 @@ class GPT2(nn.Module):
             targets.reshape(-1))
 
 
-def gpt2_small(vocab=50304, ctx=1024):
+def gpt2_small(vocab=50304, ctx=1024, **kw):
     # vocab padded 50257 -> 50304 (multiple of 64) for GEMM tile alignment
-    return GPT2(vocab=vocab, ctx=ctx)
+    return GPT2(vocab=vocab, ctx=ctx, **kw)

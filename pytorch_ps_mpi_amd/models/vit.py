@@ -6,36 +6,66 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.attn import fused_sdpa_qkv
+from ..ops.attn import fused_sdpa, fused_sdpa_qkv
 from ..ops.linear import FusedLinear
-from ..ops.ln import FusedLayerNorm
+from ..ops.ln import FusedLayerNorm, fused_gated_residual
+from ..ops.rope import AxialRotary
 
 
 class Block(nn.Module):
-    def __init__(self, dim, heads, mlp_ratio=4.0):
+    """rotary, layer_scale: as in the causal block (models/gpt2.py); rotary
+    turns by height and width."""
+
+    def __init__(self, dim, heads, mlp_ratio=4.0, rotary=None,
+                 layer_scale=None):
         super().__init__()
         self.n1 = FusedLayerNorm(dim)
         self.qkv = FusedLinear(dim, dim * 3)
         self.proj = FusedLinear(dim, dim)
         self.heads = heads
+        self.rotary = rotary
         self.n2 = FusedLayerNorm(dim)
         h = int(dim * mlp_ratio)
         self.fc1 = FusedLinear(dim, h)
         self.fc2 = FusedLinear(h, dim)
+        if layer_scale is not None:
+            self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
+            self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
 
-    def forward(self, x):
-        B, N, D = x.shape
-        qkv = self.qkv(self.n1(x)).view(B, N, 3, self.heads, D // self.heads)
-        y = fused_sdpa_qkv(qkv)  # [B, H, N, Dh]
-        y = y.transpose(1, 2).reshape(B, N, D)
-        x = x + self.proj(y)
-        x = x + self.fc2(F.gelu(self.fc1(self.n2(x))))
+    def attend(self, h, pos=None):
+        B, N, D = h.shape
+        qkv = self.qkv(h).view(B, N, 3, self.heads, D // self.heads)
+        if self.rotary is None:
+            y = fused_sdpa_qkv(qkv)  # [B, H, N, Dh]
+        else:
+            q, k, v = qkv.unbind(2)
+            q, k = self.rotary(q, k, pos)
+            y = fused_sdpa(q.transpose(1, 2), k.transpose(1, 2),
+                           v.transpose(1, 2))
+        return self.proj(y.transpose(1, 2).reshape(B, N, D))
+
+    def mlp(self, h):
+        return self.fc2(F.gelu(self.fc1(h)))
+
+    def forward(self, x, pos=None):
+        x = x + self.attend(self.n1(x), pos)
+        x = x + self.mlp(self.n2(x))
         return x
+
+    def joined(self, x, h, after, pos=None):
+        x, h = fused_gated_residual(x, self.attend(h, pos), self.n2.weight,
+                                    self.n2.bias, gate=self.g1,
+                                    eps=self.n2.eps)
+        return fused_gated_residual(x, self.mlp(h), after.weight, after.bias,
+                                    gate=self.g2, eps=after.eps)
 
 
 class ViT(nn.Module):
+    """rotary=True: patches carry their row and column by rotary positions
+    (beside the learned ones); layer_scale: see Block."""
+
     def __init__(self, img=224, patch=16, dim=768, depth=12, heads=12,
-                 num_classes=1000):
+                 num_classes=1000, rotary=False, layer_scale=None):
         super().__init__()
         # patch embedding as unfold + Linear: with stride == kernel the
         # "conv" is a pure reshape + GEMM, which keeps it on hipBLASLt
@@ -46,7 +76,21 @@ class ViT(nn.Module):
         n = (img // patch) ** 2
         self.cls = nn.Parameter(torch.zeros(1, 1, dim))
         self.pos = nn.Parameter(torch.randn(1, n + 1, dim) * 0.02)
-        self.blocks = nn.ModuleList(Block(dim, heads) for _ in range(depth))
+        rot = None
+        if rotary:
+            pairs = dim // heads // 4
+            rot = AxialRotary(dim // heads, (pairs, pairs))
+            side = torch.arange(img // patch)
+            grid = torch.stack([side.repeat_interleave(len(side)),
+                                side.repeat(len(side))]) + 1
+            # the class token stands at (0, 0)
+            self.register_buffer("grid", F.pad(grid, (1, 0)),
+                                 persistent=False)
+        self.rotary = rotary
+        self.layer_scale = layer_scale
+        self.blocks = nn.ModuleList(
+            Block(dim, heads, rotary=rot, layer_scale=layer_scale)
+            for _ in range(depth))
         self.norm = FusedLayerNorm(dim)
         self.head = nn.Linear(dim, num_classes)
 
@@ -62,10 +106,17 @@ class ViT(nn.Module):
         x = self.patch_embed(self._patchify(x))
         cls = self.cls.expand(x.shape[0], -1, -1)
         x = torch.cat([cls, x], dim=1) + self.pos
-        for blk in self.blocks:
-            x = blk(x)
-        return self.head(self.norm(x)[:, 0])
+        pos = self.grid if self.rotary else None
+        if self.layer_scale is None:
+            for blk in self.blocks:
+                x = blk(x, pos)
+            return self.head(self.norm(x)[:, 0])
+        norms = [blk.n1 for blk in self.blocks] + [self.norm]
+        h = norms[0](x)
+        for blk, after in zip(self.blocks, norms[1:]):
+            x, h = blk.joined(x, h, after, pos)
+        return self.head(h[:, 0])
 
 
-def vit_b16(num_classes=1000):
-    return ViT(dim=768, depth=12, heads=12, num_classes=num_classes)
+def vit_b16(num_classes=1000, **kw):
+    return ViT(dim=768, depth=12, heads=12, num_classes=num_classes, **kw)
