@@ -165,9 +165,10 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
 
 
 def _rows16(t):
-    """t as the kernels read it: unit d stride, rows that start at 16 bytes."""
+    """t as the kernels read it: unit d stride, rows that start at 16 bytes and
+    64 of them within 32-bit byte offsets."""
     if (t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3])
-            and t.data_ptr() % 16 == 0):
+            and t.stride(2) < 1 << 24 and t.data_ptr() % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

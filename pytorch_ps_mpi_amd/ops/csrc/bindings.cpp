@@ -852,7 +852,7 @@ static void wa_rows(const at::Tensor& t, const char* name, const at::Tensor& q,
               name, " has the wrong shape");
   TORCH_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 &&
                   t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
-                  (uintptr_t)t.data_ptr() % 16 == 0,
+                  t.stride(2) < (1 << 24) && (uintptr_t)t.data_ptr() % 16 == 0,
               name, " rows must be 16B-aligned with unit d-stride");
   for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
 }

@@ -113,41 +113,54 @@ __device__ __forceinline__ void wa_row(const __bf16* row, int half, wa_bf8* f) {
   for (int kk = 0; kk < D / 16; ++kk) f[kk] = *(const wa_bf8*)(row + kk * 16 + half * 8);
 }
 
-// A tile on its way: 64 rows of D elements by 256 threads.  Rows past the
-// length take the last one's place: what stands there is never read.
+// A tile on its way: 64 rows of D elements by 256 threads.  Whole tiles are
+// addressed by a scalar base and a 32-bit offset a lane; in the last one rows
+// past the length take the last one's place: what stands there is never read.
 template <int D>
 struct WaStage {
   static constexpr int G = D / 8, STEP = WA_BLOCK / G, CNT = WA_T / STEP;
   wa_u4 v[CNT];
   __device__ __forceinline__ void load(const __bf16* base, int64_t sN, int row0, int len) {
-    const int g = threadIdx.x % G, r = threadIdx.x / G;
+    const uint32_t g = threadIdx.x % G, r = threadIdx.x / G;
+    if (row0 + WA_T <= len) {
+      const uint32_t off = (r * (uint32_t)sN + g * 8) * 2;
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int row = min(row0 + r + i * STEP, len - 1);
-      v[i] = *(const wa_u4*)(base + row * sN + g * 8);
+      for (int i = 0; i < CNT; ++i) {
+        const char* at = (const char*)(base + (row0 + i * STEP) * sN);
+        v[i] = *(const wa_u4*)(at + off);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) {
+        const int row = min(row0 + (int)r + i * STEP, len - 1);
+        v[i] = *(const wa_u4*)(base + row * sN + g * 8);
+      }
     }
   }
-  __device__ __forceinline__ void store(__bf16* lds) const {
+  __device__ __forceinline__ static int place() {  // of v[0], in bytes
     const int g = threadIdx.x % G, r = threadIdx.x / G;
+    return r * D * 2 + ((g ^ wa_swz<D>(r)) * 16);
+  }
+  // rows STEP apart have the same swizzle: it looks at a row modulo 16
+  __device__ __forceinline__ void store(char* lds, int at) const {
+    static_assert(STEP % 16 == 0, "swizzle of rows STEP apart");
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int row = r + i * STEP;
-      *(wa_u4*)(lds + row * D + ((g ^ wa_swz<D>(row)) * 8)) = v[i];
-    }
+    for (int i = 0; i < CNT; ++i) *(wa_u4*)(lds + at + i * STEP * D * 2) = v[i];
   }
 };
 
 // Row operand: rows sub*32 + lane%32 of a tile, columns 16kk + 8*half ...
 template <int D>
 struct WaRows {
-  int base, swz, half;
+  int at[D / 16];
   __device__ __forceinline__ WaRows(int lane) {
-    base = (lane & 31) * D;
-    swz = wa_swz<D>(lane & 31);
-    half = lane >> 5;
+    const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+      at[kk] = row * D * 2 + (((2 * kk + half) ^ wa_swz<D>(row)) * 16);
   }
-  __device__ __forceinline__ wa_bf8 get(const __bf16* tile, int sub, int kk) const {
-    return *(const wa_bf8*)(tile + sub * 32 * D + base + (((2 * kk + half) ^ swz) * 8));
+  __device__ __forceinline__ wa_bf8 get(const char* tile, int sub, int kk) const {
+    return *(const wa_bf8*)(tile + at[kk] + sub * 32 * D * 2);
   }
 };
 
@@ -164,14 +177,14 @@ struct WaCols {
       for (int dt = 0; dt < D / 32; ++dt) {
         const int row = 8 * jj + 4 * half + (i >> 2);
         const int col = 32 * dt + 16 * (grp & 1) + (i & 3) * 4;
-        at[jj][dt] = row * D + ((col >> 3) ^ wa_swz<D>(row)) * 8 + (col & 7);
+        at[jj][dt] = row * D * 2 + ((col >> 3) ^ wa_swz<D>(row)) * 16 + (col & 7) * 2;
       }
   }
-  __device__ __forceinline__ wa_bf8 get(const __bf16* tile, int ks, int dt) const {
+  __device__ __forceinline__ wa_bf8 get(const char* tile, int ks, int dt) const {
     const wa_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (wa_lds_s4*)(tile + ks * 16 * D + at[0][dt]));
+        (wa_lds_s4*)(tile + at[0][dt] + ks * 16 * D * 2));
     const wa_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (wa_lds_s4*)(tile + ks * 16 * D + at[1][dt]));
+        (wa_lds_s4*)(tile + at[1][dt] + ks * 16 * D * 2));
     const wa_s8 s = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(wa_bf8, s);
   }
@@ -210,13 +223,17 @@ struct WaPlace {
   }
 };
 
+__device__ __forceinline__ int wa_wave() {  // the same for all lanes: a scalar
+  return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+
 __device__ __forceinline__ int wa_len(const WaArgs& a, int b) {
   return a.lengths ? max(0, min(a.lengths[b], a.N)) : a.N;
 }
 
 __device__ __forceinline__ WaPlace wa_place(const WaArgs& a, int gw) {
   WaPlace w;
-  const int rw = 4 / gw, rows = 32 * rw, wave = threadIdx.x >> 6;
+  const int rw = 4 / gw, rows = 32 * rw, wave = wa_wave();
   const int blocks = (a.N + rows - 1) / rows, hb = a.H / gw;
   const int u = blockIdx.x / blocks;
   // last rows first: in a short sequence they have the most keys
@@ -243,8 +260,35 @@ __device__ __forceinline__ int wa_seen(const WaArgs& a, int r0, int k0, int n) {
   return 1;
 }
 
-__device__ __forceinline__ bool wa_vis(const WaArgs& a, int i, int j) {
-  return j <= i && (i - j < a.window || j < a.sinks);
+// Of rows r0..r0+63 and keys k0..k0+31, likewise
+__device__ __forceinline__ int wa_seen_tile(const WaArgs& a, int r0, int k0) {
+  if (k0 > r0 + WA_T - 1) return 0;
+  if (k0 >= a.sinks && r0 - (k0 + 31) >= a.window) return 0;
+  if (k0 + 31 <= r0 && (r0 + WA_T - 1 - k0 < a.window || k0 + 32 <= a.sinks)) return 2;
+  return 1;
+}
+
+// Whether element t of a lane is visible; d = row - key grows by `step` with t:
+// 0 <= d < window is one unsigned comparison.
+struct WaVis {
+  int d0;         // row - key at t = 0
+  uint32_t window;
+  int sink;       // d is also visible from 0 to any size where t < sink
+  bool any_sink;  // the same for all lanes
+};
+// keys run with t (forward, dQ): d = d0 - t
+__device__ __forceinline__ bool wa_vis_key(const WaVis& v, int t) {
+  bool ok = (uint32_t)(v.d0 - t) < v.window;
+  if (v.any_sink) ok = ok || t < v.sink;
+  return ok;
+}
+__device__ __forceinline__ WaVis wa_vis_of(const WaArgs& a, int row, int k0, int half) {
+  WaVis v;
+  v.d0 = row - k0 - 4 * half;
+  v.window = (uint32_t)a.window;
+  v.any_sink = k0 < a.sinks;
+  v.sink = min(a.sinks - k0 - 4 * half, v.d0 + 1);
+  return v;
 }
 
 // ---------------------------------------------------------------------------
@@ -253,7 +297,8 @@ __device__ __forceinline__ bool wa_vis(const WaArgs& a, int i, int j) {
 
 template <int D>
 __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) {
-  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
+  constexpr int TILE = WA_T * D * 2;  // bytes; two buffers of K and V
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const WaPlace w = wa_place(a, gw);
   const int row = w.wrow + col;
@@ -271,65 +316,89 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
   wa_row<D>(a.q.p + w.b * a.q.sB + w.head * a.q.sH + min(row, w.len - 1) * a.q.sN, half, qf);
   const WaRows<D> rows(lane);
   const WaCols<D> cols(lane);
-  WaStage<D> sk, sv;
-  sk.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
-  sv.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+  const int put = WaStage<D>::place();
+  // K and V take turns in the registers of one tile on its way
+  {
+    WaStage<D> st;
+    st.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
+    st.store(lds, put);
+    st.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+    st.store(lds + TILE, put);
+  }
   const float c = a.scale * WA_LOG2E;
   float m = -3.0e38f, l = 0.0f;  // l: this half wave's keys
-  for (int it = 0; it < w.count; ++it) {
-    __bf16* tk = lds[it & 1][0];
-    __bf16* tv = lds[it & 1][1];
+  auto step = [&](int it, char* mine, char* next) {
+    char* tk = mine;
+    char* tv = mine + TILE;
     const int k0 = w.tile(it) * WA_T;
-    sk.store(tk);
-    sv.store(tv);
-    if (it + 1 < w.count) {
-      sk.load(kb, a.k.sN, w.tile(it + 1) * WA_T, w.len);
-      sv.load(vb, a.v.sN, w.tile(it + 1) * WA_T, w.len);
-    }
+    const bool more = it + 1 < w.count;
+    const int n0 = more ? w.tile(it + 1) * WA_T : 0;
     __syncthreads();
+    WaStage<D> st;
+    if (more) st.load(kb, a.k.sN, n0, w.len);
     const int seen = wa_seen(a, w.wrow, k0, WA_T);
-    if (seen == 0) continue;
     wa_f16 s[2];
+    if (seen) {
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      s[sub] = (wa_f16)(0.0f);
+      for (int sub = 0; sub < 2; ++sub) {
+        wa_bf8 f[D / 16];
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        s[sub] = wa_mfma(rows.get(tk, sub, kk), qf[kk], s[sub]);
+        for (int kk = 0; kk < D / 16; ++kk) f[kk] = rows.get(tk, sub, kk);
+        s[sub] = (wa_f16)(0.0f);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) s[sub] = wa_mfma(f[kk], qf[kk], s[sub]);
+      }
     }
-    if (seen == 1) {
+    if (more) {
+      st.store(next, put);
+      st.load(vb, a.v.sN, n0, w.len);
+    }
+    if (seen) {
+      // scaled first: the products need no quieting before the comparisons
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) s[sub] *= c;
+      if (seen == 1) {
+        const WaVis vis = wa_vis_of(a, row, k0, half);
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!wa_vis_key(vis, sub * 32 + 8 * (r / 4) + r % 4)) s[sub][r] = -INFINITY;
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+      const float mn = fmaxf(m, wa_other_max(top));
+      // weights may pass 1 by a factor of 2^8 before everything is rescaled
+      if (__any(mn > m + 8.0f)) {
+        const float f = wa_exp2(m - mn);
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) acc[t] *= f;
+        m = mn;
+      }
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = k0 + sub * 32 + 8 * (r / 4) + 4 * half + r % 4;
-          if (!wa_vis(a, row, key)) s[sub][r] = -INFINITY;
+          s[sub][r] = wa_exp2(s[sub][r] - m);
+          l += s[sub][r];
         }
-    }
-    float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
-    const float mn = fmaxf(m, wa_other_max(top) * c);
-    if (__any(mn > m)) {
-      const float f = wa_exp2(m - mn);
-      l *= f;
+      for (int ks = 0; ks < 4; ++ks) {
+        wa_bf8 f[D / 32];
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t) acc[t] *= f;
-      m = mn;
-    }
+        for (int t = 0; t < D / 32; ++t) f[t] = cols.get(tv, ks, t);
+        const wa_bf8 p = wa_operand(s[ks >> 1], ks & 1);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[sub][r] = wa_exp2(fmaf(s[sub][r], c, -m));
-        l += s[sub][r];
+        for (int t = 0; t < D / 32; ++t) acc[t] = wa_mfma(f[t], p, acc[t]);
       }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const wa_bf8 p = wa_operand(s[ks >> 1], ks & 1);
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) acc[t] = wa_mfma(cols.get(tv, ks, t), p, acc[t]);
     }
+    if (more) st.store(next + TILE, put);
+  };
+  for (int it = 0; it < w.count; it += 2) {
+    step(it, lds, lds + 2 * TILE);
+    if (it + 1 < w.count) step(it + 1, lds + 2 * TILE, lds);
   }
   l = wa_other_sum(l);
   const bool in = row < w.len;
@@ -347,7 +416,8 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
 
 template <int D>
 __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
-  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
+  constexpr int TILE = WA_T * D * 2;  // bytes; two buffers of K and V
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const WaPlace w = wa_place(a, gw);
   const int row = w.wrow + col;
@@ -382,47 +452,60 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
   if (in && half == 0) a.delta[stat] = delta;
   const WaRows<D> rows(lane);
   const WaCols<D> cols(lane);
-  WaStage<D> sk, sv;
-  sk.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
-  sv.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+  const int put = WaStage<D>::place();
+  {
+    WaStage<D> st;
+    st.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
+    st.store(lds, put);
+    st.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
+    st.store(lds + TILE, put);
+  }
   const float c = a.scale * WA_LOG2E;
-  for (int it = 0; it < w.count; ++it) {
-    __bf16* tk = lds[it & 1][0];
-    __bf16* tv = lds[it & 1][1];
+  auto step = [&](int it, char* mine, char* next) {
+    char* tk = mine;
+    char* tv = mine + TILE;
     const int k0 = w.tile(it) * WA_T;
-    sk.store(tk);
-    sv.store(tv);
-    if (it + 1 < w.count) {
-      sk.load(kb, a.k.sN, w.tile(it + 1) * WA_T, w.len);
-      sv.load(vb, a.v.sN, w.tile(it + 1) * WA_T, w.len);
-    }
+    const bool more = it + 1 < w.count;
+    const int n0 = more ? w.tile(it + 1) * WA_T : 0;
     __syncthreads();
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
+      WaStage<D> st;
+      if (more) st.load(sub ? vb : kb, sub ? a.v.sN : a.k.sN, n0, w.len);
       const int seen = wa_seen(a, w.wrow, k0 + sub * 32, 32);
-      if (seen == 0) continue;
-      wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
+      if (seen) {
+        wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        s = wa_mfma(rows.get(tk, sub, kk), qf[kk], s);
-        p = wa_mfma(rows.get(tv, sub, kk), gf[kk], p);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          s = wa_mfma(rows.get(tk, sub, kk), qf[kk], s);
+          p = wa_mfma(rows.get(tv, sub, kk), gf[kk], p);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = wa_exp2(fmaf(s[r], c, -lse));
+        if (seen == 1) {
+          const WaVis vis = wa_vis_of(a, row, k0 + sub * 32, half);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!wa_vis_key(vis, 8 * (r / 4) + r % 4)) s[r] = 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= p[r] - delta;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          wa_bf8 f[D / 32];
+#pragma unroll
+          for (int t = 0; t < D / 32; ++t) f[t] = cols.get(tk, sub * 2 + ks, t);
+          const wa_bf8 d = wa_operand(s, ks);
+#pragma unroll
+          for (int t = 0; t < D / 32; ++t) acc[t] = wa_mfma(f[t], d, acc[t]);
+        }
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float e = wa_exp2(fmaf(s[r], c, -lse));
-        if (seen == 1 &&
-            !wa_vis(a, row, k0 + sub * 32 + 8 * (r / 4) + 4 * half + r % 4))
-          e = 0.0f;
-        s[r] = e * (p[r] - delta);
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const wa_bf8 d = wa_operand(s, ks);
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t)
-          acc[t] = wa_mfma(cols.get(tk, sub * 2 + ks, t), d, acc[t]);
-      }
+      if (more) st.store(next + sub * TILE, put);
     }
+  };
+  for (int it = 0; it < w.count; it += 2) {
+    step(it, lds, lds + 2 * TILE);
+    if (it + 1 < w.count) step(it + 1, lds + 2 * TILE, lds);
   }
   wa_store<D>(out, acc, a.scale, half, in);
   if (!in && row < a.N)
@@ -437,11 +520,13 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
 // window of a block of first tokens.
 
 template <int D>
-__global__ void __launch_bounds__(WA_BLOCK, 1) k_wa_dkv(const WaArgs a) {
-  __shared__ __attribute__((aligned(16))) __bf16 lds[2][2][WA_T * D];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][WA_T];
+__global__ void __launch_bounds__(WA_BLOCK, D == 64 ? 2 : 1) k_wa_dkv(const WaArgs a) {
+  constexpr int TILE = WA_T * D * 2;
+  // two buffers of Q, dO and the rows' statistics
+  __shared__ __attribute__((aligned(16))) char lds[2 * (2 * TILE + 2 * WA_T * 4)];
+  constexpr int BUF = 2 * TILE + 2 * WA_T * 4;
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-  const int wave = threadIdx.x >> 6;
+  const int wave = wa_wave();
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
   const int nsb = a.chunks ? (a.sinks + WA_KB - 1) / WA_KB : 0;
   const int per = nkb + nsb * a.chunks;
@@ -485,11 +570,14 @@ __global__ void __launch_bounds__(WA_BLOCK, 1) k_wa_dkv(const WaArgs a) {
     wa_row<D>(a.v.p + b * a.v.sB + kv * a.v.sH + at * a.v.sN, half, vf);
     const WaRows<D> rows(lane);
     const WaCols<D> cols(lane);
+    const int put = WaStage<D>::place();
     WaStage<D> sq, sg;
     float sl = 0.0f, sd = 0.0f;
     const float c = a.scale * WA_LOG2E;
-    auto load = [&](int it) {
-      const int head = kv * G + it / total, r0 = (t0 + it % total) * WA_T;
+    const bool sinkkey = key < a.sinks;
+    int head = kv * G + it0 / total, tile = it0 % total;  // what is loaded next
+    auto load = [&]() {
+      const int r0 = (t0 + tile) * WA_T;
       sq.load(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN, r0, len);
       sg.load(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN, r0, len);
       if (threadIdx.x < WA_T) {
@@ -499,56 +587,73 @@ __global__ void __launch_bounds__(WA_BLOCK, 1) k_wa_dkv(const WaArgs a) {
         sd = a.delta[i];
       }
     };
-    load(it0);
-    for (int it = it0; it < it1; ++it) {
-      const int buf = (it - it0) & 1;
-      __bf16* tq = lds[buf][0];
-      __bf16* tg = lds[buf][1];
-      sq.store(tq);
-      sg.store(tg);
+    load();
+    int row0 = (t0 + tile) * WA_T;  // of the tile that is stored next
+    auto step = [&](int it, char* buf) {
+      char* tq = buf;
+      char* tg = buf + TILE;
+      float* stat = (float*)(buf + 2 * TILE);
+      const int r0 = row0;
+      sq.store(tq, put);
+      sg.store(tg, put);
       if (threadIdx.x < WA_T) {
-        stat[buf][0][threadIdx.x] = sl;
-        stat[buf][1][threadIdx.x] = sd;
+        stat[threadIdx.x] = sl;
+        stat[WA_T + threadIdx.x] = sd;
       }
-      const int r0 = (t0 + it % total) * WA_T;
-      if (it + 1 < it1) load(it + 1);
+      if (it + 1 < it1) {
+        if (++tile == total) {
+          tile = 0;
+          ++head;
+        }
+        row0 = (t0 + tile) * WA_T;
+        load();
+      }
       __syncthreads();
+      const int seen = wa_seen_tile(a, r0, wk);
+      if (seen == 0) return;
+      wa_f16 s[2], p[2];
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        const int rs = r0 + sub * 32;
-        const int seen = wa_seen(a, rs, wk, 32);
-        if (seen == 0) continue;
-        wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
+        s[sub] = p[sub] = (wa_f16)(0.0f);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          s = wa_mfma(rows.get(tq, sub, kk), kf[kk], s);
-          p = wa_mfma(rows.get(tg, sub, kk), vf[kk], p);
-        }
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int r = sub * 32 + 8 * r4 + 4 * half;
-          const float4 ls = *(const float4*)&stat[buf][0][r];
-          const float4 de = *(const float4*)&stat[buf][1][r];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float lj = j == 0 ? ls.x : j == 1 ? ls.y : j == 2 ? ls.z : ls.w;
-            const float dj = j == 0 ? de.x : j == 1 ? de.y : j == 2 ? de.z : de.w;
-            float e = wa_exp2(fmaf(s[4 * r4 + j], c, -lj));
-            if (seen == 1 && !wa_vis(a, r0 + r + j, key)) e = 0.0f;
-            s[4 * r4 + j] = e;
-            p[4 * r4 + j] = e * (p[4 * r4 + j] - dj);
-          }
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const wa_bf8 pf = wa_operand(s, ks), df = wa_operand(p, ks);
-#pragma unroll
-          for (int t = 0; t < D / 32; ++t) {
-            av[t] = wa_mfma(cols.get(tg, sub * 2 + ks, t), pf, av[t]);
-            ak[t] = wa_mfma(cols.get(tq, sub * 2 + ks, t), df, ak[t]);
-          }
+          s[sub] = wa_mfma(rows.get(tq, sub, kk), kf[kk], s[sub]);
+          p[sub] = wa_mfma(rows.get(tg, sub, kk), vf[kk], p[sub]);
         }
       }
+      const int d0 = r0 + 4 * half - key;  // row - key at t = 0
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int t0 = sub * 32 + 8 * r4;
+          const float4 ls = *(const float4*)(stat + t0 + 4 * half);
+          const float4 de = *(const float4*)(stat + WA_T + t0 + 4 * half);
+          const float lj[4] = {ls.x, ls.y, ls.z, ls.w}, dj[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float e = wa_exp2(fmaf(s[sub][4 * r4 + j], c, -lj[j]));
+            if (seen == 1) {
+              const int d = d0 + t0 + j;
+              if (!((uint32_t)d < (uint32_t)a.window || (sinkkey && d >= 0))) e = 0.0f;
+            }
+            s[sub][4 * r4 + j] = e;
+            p[sub][4 * r4 + j] = e * (p[sub][4 * r4 + j] - dj[j]);
+          }
+        }
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const wa_bf8 pf = wa_operand(s[ks >> 1], ks & 1), df = wa_operand(p[ks >> 1], ks & 1);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) {
+          av[t] = wa_mfma(cols.get(tg, ks, t), pf, av[t]);
+          ak[t] = wa_mfma(cols.get(tq, ks, t), df, ak[t]);
+        }
+      }
+    };
+    for (int it = it0; it < it1; it += 2) {
+      step(it, lds);
+      if (it + 1 < it1) step(it + 1, lds + BUF);
     }
   }
   if (sinkblk && a.chunks) {
