@@ -199,7 +199,8 @@ class _WindowSDPA(torch.autograd.Function):
                               device=q.device).transpose(1, 2)
                   for _ in range(2))
         delta = torch.empty_like(lse)
-        part = torch.empty(_EXT.wa_part_floats(B, KV, N, D, window, sinks),
+        part = torch.empty(_EXT.wa_part_floats(B, H, KV, N, D, window,
+                                               sinks),
                            dtype=torch.float32, device=q.device)
         _EXT.wa_bwd(q, k, v, o, _rows16(dout), lse, delta, dq, dk, dv, part,
                     lengths, window, sinks, scale)

@@ -35,7 +35,7 @@ int ps_join_bwd(void* stream, void* const* t, float* const* stats,
                 void* const* sums, float* part, int bf16, int64_t groups,
                 int64_t rows, int64_t D, int layer, int gate_kind,
                 int64_t gate_step, float scale);
-int64_t ps_wa_part_floats(int64_t B, int64_t KV, int64_t N, int64_t D,
+int64_t ps_wa_part_floats(int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
                           int64_t window, int64_t sinks);
 int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
               void* o, float* lse, const int32_t* lengths, const int64_t* st,
@@ -901,9 +901,9 @@ void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
            "wa_fwd");
 }
 
-int64_t wa_part_floats(int64_t B, int64_t KV, int64_t N, int64_t D,
+int64_t wa_part_floats(int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
                        int64_t window, int64_t sinks) {
-  return ps_wa_part_floats(B, KV, N, D, window, sinks);
+  return ps_wa_part_floats(B, H, KV, N, D, window, sinks);
 }
 
 void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
@@ -925,7 +925,7 @@ void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
   wa_stat(delta, q);
   check_flat(part, at::kFloat, "part");
   check_same_device(q, part, "part");
-  TORCH_CHECK(part.numel() >= ps_wa_part_floats(q.size(0), k.size(1),
+  TORCH_CHECK(part.numel() >= ps_wa_part_floats(q.size(0), q.size(1), k.size(1),
                                                 q.size(2), q.size(3), window,
                                                 sinks),
               "part too small");
