@@ -246,13 +246,20 @@ __device__ __forceinline__ int wa_len(const WaArgs& a, int b) {
   return a.lengths ? max(0, min(a.lengths[b], a.N)) : a.N;
 }
 
+// Blocks go to the 8 XCDs in turn, each with an L2 of its own: give every XCD a
+// stretch of neighbouring blocks, which read the same tiles.
+__device__ __forceinline__ int wa_block() {
+  const int n = gridDim.x, x = blockIdx.x & 7;
+  return x * (n >> 3) + min(x, n & 7) + (blockIdx.x >> 3);
+}
+
 __device__ __forceinline__ WaPlace wa_place(const WaArgs& a, int gw) {
   WaPlace w;
   const int rw = 4 / gw, rows = 32 * rw, wave = wa_wave();
   const int blocks = (a.N + rows - 1) / rows, hb = a.H / gw;
-  const int u = blockIdx.x / blocks;
+  const int id = wa_block(), u = id / blocks;
   // last rows first: in a short sequence they have the most keys
-  const int blk = blocks - 1 - (blockIdx.x - u * blocks);
+  const int blk = blocks - 1 - (id - u * blocks);
   w.b = u / hb;
   const int h0 = (u - w.b * hb) * gw;
   w.head = h0 + wave % gw;
@@ -574,7 +581,7 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = wa_wave(), part = PARTS == 1 ? 0 : wave >> 2;
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
-  const int u = blockIdx.x / nkb, k0 = (blockIdx.x - u * nkb) * WA_KB;
+  const int id = wa_block(), u = id / nkb, k0 = (id - u * nkb) * WA_KB;
   const int b = u / a.KV, kv = u - b * a.KV, G = a.H / a.KV;
   const int len = wa_len(a, b);
   // the rows, in tiles, of each head: the window's
