@@ -164,49 +164,6 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
     return (p @ vf).to(q.dtype)
 
 
-def _rows16(t):
-    """t as the kernels read it: unit d stride, rows that start at 16 bytes and
-    64 of them within 32-bit byte offsets."""
-    if (t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3])
-            and t.stride(2) < 1 << 24 and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-class _WindowSDPA(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, lengths, scale):
-        q, k, v = (_rows16(t) for t in (q, k, v))
-        B, H, N, D = q.shape
-        # heads stand behind rows: what follows is a projection of all heads
-        o = torch.empty(B, N, H, D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device)
-        o = o.transpose(1, 2)
-        _EXT.wa_fwd(q, k, v, o, lse, lengths, window, sinks, scale)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
-        ctx.cfg = (window, sinks, scale)
-        return o
-
-    @staticmethod
-    def backward(ctx, dout):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
-        window, sinks, scale = ctx.cfg
-        B, H, N, D = q.shape
-        KV = k.shape[1]
-        dq = torch.empty(B, N, H, D, dtype=q.dtype,
-                         device=q.device).transpose(1, 2)
-        dk, dv = (torch.empty(B, N, KV, D, dtype=q.dtype,
-                              device=q.device).transpose(1, 2)
-                  for _ in range(2))
-        delta = torch.empty_like(lse)
-        part = torch.empty(_EXT.wa_part_floats(B, H, KV, N, D, window,
-                                               sinks),
-                           dtype=torch.float32, device=q.device)
-        _EXT.wa_bwd(q, k, v, o, _rows16(dout), lse, delta, dq, dk, dv, part,
-                    lengths, window, sinks, scale)
-        return dq, dk, dv, None, None, None, None
-
-
 def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):
     """Causal attention in which row i sees key j <= i if ``i - j < window`` or
     ``j < sinks`` (the first tokens stay visible).
@@ -249,7 +206,5 @@ def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):
         raise ValueError("scale must be positive and finite")
     if (_require_ext(q) and q.dtype == torch.bfloat16 and D in (64, 128)
             and q.numel()):
-        if lengths is not None:
-            lengths = lengths.contiguous()
-        return _WindowSDPA.apply(q, k, v, window, sinks, lengths, scale)
+        return _EXT.window_sdpa(q, k, v, window, sinks, lengths, scale)
     return _window_plain(q, k, v, window, sinks, lengths, scale)

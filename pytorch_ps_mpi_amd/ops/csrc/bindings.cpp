@@ -298,18 +298,24 @@ int float_kind(const at::Tensor& t, const char* name) {
   return st == at::kBFloat16 ? 0 : st == at::kHalf ? 1 : 2;
 }
 
-void rope(at::Tensor q, at::Tensor k, at::Tensor yq, at::Tensor yk,
-          at::Tensor pos, std::vector<int64_t> start, at::Tensor rev,
-          bool inter, bool backward) {
+// No second derivatives: a backward pass of these functions is not recorded.
+void first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what,
+              " has no second derivative (create_graph=True)");
+}
+
+// q, k [B, N, heads, D] turned by positions [axes, B, N]; `rev`: revolutions a
+// position for each pair (host, fp64), `start`: first pair of axes 1 to 3.
+std::vector<at::Tensor> rope_apply(at::Tensor q, at::Tensor k,
+                                   const at::Tensor& pos,
+                                   const std::vector<int64_t>& start,
+                                   const at::Tensor& rev, bool inter,
+                                   bool backward) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4, "q, k: 4-D on GPU");
-  TORCH_CHECK(q.stride(3) == 1 && k.stride(3) == 1, "unit last stride");
   TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
                   q.size(3) == k.size(3) && k.scalar_type() == q.scalar_type(),
               "q and k differ in B, N, D or type");
-  TORCH_CHECK(yq.sizes() == q.sizes() && yk.sizes() == k.sizes(), "out sizes");
-  check_flat(yq, q.scalar_type(), "yq");
-  check_flat(yk, q.scalar_type(), "yk");
-  for (const auto& t : {k, yq, yk, pos}) check_same_device(q, t, "rope input");
+  for (const auto& t : {k, pos}) check_same_device(q, t, "rope input");
   TORCH_CHECK(pos.dim() == 3 && pos.size(1) == q.size(0) &&
                   pos.size(2) == q.size(1), "positions [axes, B, N]");
   TORCH_CHECK(pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt,
@@ -324,10 +330,14 @@ void rope(at::Tensor q, at::Tensor k, at::Tensor yq, at::Tensor yk,
     axes += first[i] < P;
   }
   TORCH_CHECK(pos.size(0) >= axes, "a position for each axis");
+  const c10::DeviceGuard guard(q.device());
+  if (q.stride(3) != 1) q = q.contiguous();
+  if (k.stride(3) != 1) k = k.contiguous();
+  auto yq = at::empty(q.sizes(), q.options());
+  auto yk = at::empty(k.sizes(), k.options());
   const int64_t strides[9] = {q.stride(0), q.stride(1), q.stride(2),
                               k.stride(0), k.stride(1), k.stride(2),
                               pos.stride(0), pos.stride(1), pos.stride(2)};
-  const c10::DeviceGuard guard(q.device());
   throw_on(ps_rope(cur_stream(q), q.data_ptr(), k.data_ptr(), yq.data_ptr(),
                    yk.data_ptr(), pos.data_ptr(),
                    pos.scalar_type() == at::kLong, float_kind(q, "q"), strides,
@@ -335,6 +345,37 @@ void rope(at::Tensor q, at::Tensor k, at::Tensor yq, at::Tensor yk,
                    (int)q.size(3), P, first, rev.data_ptr<double>(),
                    inter ? 1 : 0, backward ? 1 : 0),
            "rope");
+  return {yq, yk};
+}
+
+// The backward pass is the turn by the opposite angles.
+struct Rope : torch::autograd::Function<Rope> {
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+      const at::Tensor& k, const at::Tensor& pos, std::vector<int64_t> start,
+      const at::Tensor& rev, bool inter) {
+    ctx->save_for_backward({pos, rev});
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["inter"] = inter;
+    return rope_apply(q, k, pos, start, rev, inter, false);
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list g) {
+    first_order("AxialRotary");
+    const auto saved = ctx->get_saved_variables();
+    auto d = rope_apply(g[0], g[1], saved[0],
+                        ctx->saved_data["start"].toIntVector(), saved[1],
+                        ctx->saved_data["inter"].toBool(), true);
+    return {d[0], d[1], at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+std::vector<at::Tensor> rope(at::Tensor q, at::Tensor k, at::Tensor pos,
+                             std::vector<int64_t> start, at::Tensor rev,
+                             bool inter) {
+  return Rope::apply(q, k, pos, start, rev, inter);
 }
 
 // ---- norms before and after a block with its gate and residual ------------
@@ -369,10 +410,6 @@ int64_t join_gate(int64_t kind, int64_t step, int64_t groups, int64_t rows,
                   int64_t D) {
   TORCH_CHECK(kind >= 0 && kind <= 2 && (step == 0 || step == D), "gate kind");
   return kind == 2 ? groups * rows * D : step ? groups * D : D;
-}
-
-int64_t join_blocks(int64_t groups, int64_t rows, int64_t D) {
-  return ps_join_blocks(groups, rows, D, 1);
 }
 
 // t: x, u, w, b, pw, pb, gate, y, h
@@ -429,6 +466,95 @@ void join_bwd(OptTensors t, at::Tensor stats, OptTensors sums, at::Tensor part,
                        is_bf16(u), groups, rows, D, layer ? 1 : 0,
                        (int)gate_kind, gate_step, (float)scale),
            "join_bwd");
+}
+
+// groups, rows: the gate's vector is one of `groups`, each for `rows` rows;
+// gate_kind 0 none, 1 vector, 2 x's shape.
+struct GatedResidual : torch::autograd::Function<GatedResidual> {
+  using Opt = c10::optional<at::Tensor>;
+  static at::Tensor dense(const Opt& t) {
+    return t.has_value() ? t->contiguous() : at::Tensor();
+  }
+  static Opt opt(const at::Tensor& t) {
+    return t.defined() ? Opt(t) : Opt();
+  }
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const at::Tensor& x_,
+      const at::Tensor& u_, const at::Tensor& w_, const Opt& b_,
+      const Opt& gate_, const Opt& pw_, const Opt& pb_, double scale,
+      double eps, bool layer, int64_t groups, int64_t gate_kind) {
+    const c10::DeviceGuard guard(x_.device());
+    const auto x = x_.contiguous(), u = u_.contiguous(), w = w_.contiguous();
+    const auto b = dense(b_), gate = dense(gate_), pw = dense(pw_),
+               pb = dense(pb_);
+    const int64_t D = x.size(-1), rows = x.numel() / D / groups;
+    const int64_t step = gate_kind == 1 && groups > 1 ? D : 0;
+    auto y = at::empty_like(x), h = at::empty_like(x);
+    auto stats = at::empty({pw.defined() ? 4 : 2, groups * rows},
+                           x.options().dtype(at::kFloat));
+    join_fwd({x, u, w, opt(b), opt(pw), opt(pb), opt(gate), y, h}, stats,
+             groups, rows, D, layer, gate_kind, step, scale, eps);
+    ctx->save_for_backward({y, u, w, gate, pw, pb, stats});
+    ctx->saved_data["cfg"] =
+        std::vector<int64_t>{groups, rows, D, layer, gate_kind, step,
+                             b.defined()};
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return {y, h};
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list g) {
+    first_order("fused_gated_residual");
+    torch::autograd::variable_list out(12);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const auto &y = s[0], &u = s[1], &w = s[2], &gate = s[3], &pw = s[4],
+               &pb = s[5], &stats = s[6];
+    const auto cfg = ctx->saved_data["cfg"].toIntVector();
+    const int64_t groups = cfg[0], rows = cfg[1], D = cfg[2], kind = cfg[4];
+    const c10::DeviceGuard guard(y.device());
+    const Opt dy = g[0].defined() ? Opt(g[0].contiguous()) : Opt();
+    const Opt dh = g[1].defined() ? Opt(g[1].contiguous()) : Opt();
+    // inputs that are there, in order: x, u, w, b, gate, pw, pb
+    const bool there[7] = {true, true, true, cfg[6] != 0, gate.defined(),
+                           pw.defined(), pb.defined()};
+    bool need[7];
+    size_t edge = 0;
+    for (int i = 0; i < 7; ++i)
+      need[i] = there[i] && ctx->needs_input_grad(edge++);
+    out[0] = at::empty_like(y);
+    out[1] = at::empty_like(u);
+    // without dh the last norm's parameters get no gradient
+    if (need[2] && dh) out[2] = at::empty_like(w);
+    if (need[3] && dh) out[3] = at::empty_like(w);
+    if (need[4]) out[4] = at::empty_like(gate);
+    if (need[5]) out[5] = at::empty_like(pw);
+    if (need[6]) out[6] = at::empty_like(pb);
+    const Opt vec = kind == 1 ? opt(out[4]) : Opt();
+    int64_t slots = vec.has_value();
+    for (int i : {2, 3, 5, 6}) slots += out[i].defined();
+    auto part = at::empty({groups * ps_join_blocks(groups, rows, D, 1) *
+                           slots * D},
+                          y.options().dtype(at::kFloat));
+    join_bwd({u, w, opt(pw), opt(pb), opt(gate), y, dy, dh, out[0], out[1],
+              kind == 2 ? opt(out[4]) : Opt()},
+             stats, {opt(out[2]), opt(out[3]), vec, opt(out[5]), opt(out[6])},
+             part, groups, rows, D, cfg[3] != 0, kind, cfg[5],
+             ctx->saved_data["scale"].toDouble());
+    if (!need[0]) out[0] = at::Tensor();
+    if (!need[1]) out[1] = at::Tensor();
+    return out;
+  }
+};
+
+std::vector<at::Tensor> gated_residual(
+    at::Tensor x, at::Tensor u, at::Tensor w, c10::optional<at::Tensor> b,
+    c10::optional<at::Tensor> gate, c10::optional<at::Tensor> pw,
+    c10::optional<at::Tensor> pb, double scale, double eps, bool layer,
+    int64_t groups, int64_t gate_kind) {
+  return GatedResidual::apply(x, u, w, b, gate, pw, pb, scale, eps, layer,
+                              groups, gate_kind);
 }
 
 void reduce_accum(at::Tensor dst, std::vector<at::Tensor> srcs, double scale,
@@ -842,7 +968,7 @@ void fa_selfcheck(at::Tensor a, at::Tensor b, at::Tensor c) {
 
 // ---- attention with a sliding window and visible first tokens -------------
 
-static void wa_rows(const at::Tensor& t, const char* name, const at::Tensor& q,
+static void wa_check(const at::Tensor& t, const char* name, const at::Tensor& q,
                     int64_t heads, int64_t* st) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4,
               name, " must be 4-D bf16 on GPU");
@@ -861,7 +987,7 @@ static void wa_rows(const at::Tensor& t, const char* name, const at::Tensor& q,
 static void wa_out(const at::Tensor& t, const char* name, const at::Tensor& q,
                    int64_t heads) {
   int64_t st[3];
-  wa_rows(t, name, q, heads, st);
+  wa_check(t, name, q, heads, st);
   TORCH_CHECK(t.transpose(1, 2).is_contiguous(), name,
               " must be stored with heads behind rows");
 }
@@ -887,9 +1013,9 @@ void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
             int64_t sinks, double scale) {
   int64_t st[15] = {0};
   TORCH_CHECK(k.dim() == 4 && q.dim() == 4, "q, k must be 4-D");
-  wa_rows(q, "q", q, q.size(1), st);
-  wa_rows(k, "k", q, k.size(1), st + 3);
-  wa_rows(v, "v", q, k.size(1), st + 6);
+  wa_check(q, "q", q, q.size(1), st);
+  wa_check(k, "k", q, k.size(1), st + 3);
+  wa_check(v, "v", q, k.size(1), st + 6);
   wa_out(o, "o", q, q.size(1));
   wa_stat(lse, q);
   const int32_t* len = wa_lengths(lengths, q);
@@ -901,11 +1027,6 @@ void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
            "wa_fwd");
 }
 
-int64_t wa_part_floats(int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
-                       int64_t window, int64_t sinks) {
-  return ps_wa_part_floats(B, H, KV, N, D, window, sinks);
-}
-
 void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
             at::Tensor go, at::Tensor lse, at::Tensor delta, at::Tensor dq,
             at::Tensor dk, at::Tensor dv, at::Tensor part,
@@ -913,11 +1034,11 @@ void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
             double scale) {
   int64_t st[15];
   TORCH_CHECK(k.dim() == 4 && q.dim() == 4, "q, k must be 4-D");
-  wa_rows(q, "q", q, q.size(1), st);
-  wa_rows(k, "k", q, k.size(1), st + 3);
-  wa_rows(v, "v", q, k.size(1), st + 6);
-  wa_rows(o, "o", q, q.size(1), st + 9);
-  wa_rows(go, "dout", q, q.size(1), st + 12);
+  wa_check(q, "q", q, q.size(1), st);
+  wa_check(k, "k", q, k.size(1), st + 3);
+  wa_check(v, "v", q, k.size(1), st + 6);
+  wa_check(o, "o", q, q.size(1), st + 9);
+  wa_check(go, "dout", q, q.size(1), st + 12);
   wa_out(dq, "dq", q, q.size(1));
   wa_out(dk, "dk", q, k.size(1));
   wa_out(dv, "dv", q, k.size(1));
@@ -940,15 +1061,88 @@ void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
            "wa_bwd");
 }
 
+// t as the kernels read it: unit d stride, rows that start at 16 bytes and 64
+// of them within 32-bit byte offsets.
+static at::Tensor wa_rows16(const at::Tensor& t) {
+  if (t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+      t.stride(2) % 8 == 0 && t.stride(2) < (1 << 24) &&
+      (uintptr_t)t.data_ptr() % 16 == 0)
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
+// [B, heads, N, D] stored with heads behind rows: what follows is a projection
+// of all heads
+static at::Tensor wa_empty(int64_t B, int64_t heads, int64_t N, int64_t D,
+                           const at::Tensor& like) {
+  return at::empty_strided({B, heads, N, D}, {N * heads * D, D, heads * D, 1},
+                           like.options());
+}
+
+struct WindowSdpa : torch::autograd::Function<WindowSdpa> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& q_, const at::Tensor& k_,
+                            const at::Tensor& v_,
+                            const c10::optional<at::Tensor>& lengths,
+                            int64_t window, int64_t sinks, double scale) {
+    TORCH_CHECK(q_.is_cuda() && q_.dim() == 4 && k_.dim() == 4 &&
+                    v_.dim() == 4, "q, k, v must be 4-D on GPU");
+    const c10::DeviceGuard guard(q_.device());
+    const auto q = wa_rows16(q_), k = wa_rows16(k_), v = wa_rows16(v_);
+    auto o = wa_empty(q.size(0), q.size(1), q.size(2), q.size(3), q);
+    auto lse = at::empty({q.size(0), q.size(1), q.size(2)},
+                         q.options().dtype(at::kFloat));
+    const at::Tensor len = lengths.has_value() ? lengths->contiguous()
+                                               : at::Tensor();
+    wa_fwd(q, k, v, o, lse, len.defined() ? c10::optional<at::Tensor>(len)
+                                          : c10::optional<at::Tensor>(),
+           window, sinks, scale);
+    ctx->save_for_backward({q, k, v, o, lse, len});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list g) {
+    first_order("fused_window_sdpa");
+    const auto s = ctx->get_saved_variables();
+    const auto &q = s[0], &k = s[1];
+    const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3),
+                  KV = k.size(1);
+    const int64_t window = ctx->saved_data["window"].toInt(),
+                  sinks = ctx->saved_data["sinks"].toInt();
+    const c10::DeviceGuard guard(q.device());
+    auto dq = wa_empty(B, H, N, D, q), dk = wa_empty(B, KV, N, D, q),
+         dv = wa_empty(B, KV, N, D, q);
+    auto delta = at::empty_like(s[4]);
+    auto part = at::empty({ps_wa_part_floats(B, H, KV, N, D, window, sinks)},
+                          q.options().dtype(at::kFloat));
+    wa_bwd(q, k, s[2], s[3], wa_rows16(g[0]), s[4], delta, dq, dk, dv, part,
+           s[5].defined() ? c10::optional<at::Tensor>(s[5])
+                          : c10::optional<at::Tensor>(),
+           window, sinks, ctx->saved_data["scale"].toDouble());
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+static at::Tensor window_sdpa(at::Tensor q, at::Tensor k, at::Tensor v,
+                              int64_t window, int64_t sinks,
+                              c10::optional<at::Tensor> lengths,
+                              double scale) {
+  return WindowSdpa::apply(q, k, v, lengths, window, sinks, scale);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
   m.def("fa_fwd", &fa_fwd, "MFMA-tiled flash attention forward");
   m.def("fa_bwd", &fa_bwd, "MFMA-tiled flash attention backward");
   m.def("fa_selfcheck", &fa_selfcheck, "16x16x32 MFMA fragment-layout check");
-  m.def("wa_fwd", &wa_fwd, "causal attention, sliding window and sinks");
-  m.def("wa_bwd", &wa_bwd);
-  m.def("wa_part_floats", &wa_part_floats);
+  m.def("window_sdpa", &window_sdpa,
+        "causal attention, sliding window and sinks, with its gradient");
   m.def("topk_encode_thresh", &topk_encode_thresh,
         "variable-k magnitude-threshold select (k_used -> device header)");
   m.def("colsum", &colsum, "column sum (bias grads)");
@@ -972,9 +1166,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "AdamW over packed fp32 buffers, states in 32 or 8 bits");
   m.def("state8_values", &state8_values, "values that 8-bit codes stand for");
   m.def("rope", &rope, "rotary positions with several axes, q and k at once");
-  m.def("join_blocks", &join_blocks);
-  m.def("join_fwd", &join_fwd, "post norm, gate, residual, pre norm");
-  m.def("join_bwd", &join_bwd);
+  m.def("gated_residual", &gated_residual,
+        "post norm, gate, residual, pre norm, with their gradients");
   m.def("reduce_accum", &reduce_accum, "dst = beta*dst + scale*sum(srcs)");
   m.def("f32_to_bf16", &f32_to_bf16, "flat cast");
   m.def("bf16_to_f32", &bf16_to_f32, "flat cast");

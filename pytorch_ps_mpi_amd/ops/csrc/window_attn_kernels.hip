@@ -48,6 +48,8 @@ typedef __attribute__((ext_vector_type(8))) short wa_s8;
 typedef __attribute__((ext_vector_type(16))) float wa_f16;
 typedef __attribute__((ext_vector_type(4))) uint32_t wa_u4;
 typedef __attribute__((address_space(3))) wa_s4 wa_lds_s4;
+typedef __attribute__((address_space(3))) void wa_lds;
+typedef __attribute__((address_space(1))) const void wa_mem;
 
 #define WA_BLOCK 256
 #define WA_T 64           // rows of a tile
@@ -94,6 +96,19 @@ __device__ __forceinline__ void wa_feed() {
   }
 }
 
+// As wa_feed, with VALUS vector instructions behind each matrix instruction.
+template <int MFMAS, int READS, int AHEAD, int EACH, int VALUS>
+__device__ __forceinline__ void wa_mix() {
+  constexpr int VALU = 0x002, MFMA = 0x008, DS_READ = 0x100;
+  __builtin_amdgcn_sched_group_barrier(DS_READ, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+    if (AHEAD + i * EACH < READS) __builtin_amdgcn_sched_group_barrier(DS_READ, EACH, 0);
+    __builtin_amdgcn_sched_group_barrier(VALU, VALUS, 0);
+  }
+}
+
 __device__ __forceinline__ float wa_exp2(float x) {
   return __builtin_amdgcn_exp2f(x);
 }
@@ -128,39 +143,40 @@ __device__ __forceinline__ void wa_row(const __bf16* row, int half, wa_bf8* f) {
   for (int kk = 0; kk < D / 16; ++kk) f[kk] = *(const wa_bf8*)(row + kk * 16 + half * 8);
 }
 
-// A tile on its way: 64 rows of D elements by 256 threads.  Whole tiles are
-// addressed by a scalar base and a 32-bit offset a lane; in the last one rows
-// past the length take the last one's place: what stands there is never read.
-template <int D, int NT = WA_BLOCK>
-struct WaStage {
-  static constexpr int G = D / 8, STEP = NT / G, CNT = WA_T / STEP;
-  wa_u4 v[CNT];
-  __device__ __forceinline__ void load(const __bf16* base, int64_t sN, int row0, int len) {
-    const uint32_t g = threadIdx.x % G, r = threadIdx.x / G;
-    if (row0 + WA_T <= len) {
-      const uint32_t off = (r * (uint32_t)sN + g * 8) * 2;
+// A tile on its way from memory to LDS, without registers: each of NW waves
+// moves pieces of 1 KB, lane i to the piece's 16 bytes number i; the swizzle is
+// on the side of memory.  Whole tiles are addressed by a scalar base and a
+// 32-bit offset a lane; in the last one rows past the length take the last
+// one's place: what stands there is never read.
+template <int D, int NW>
+struct WaMove {
+  static constexpr int G = D / 8, R = 64 / G, CNT = WA_T / R / NW;
+  int first;      // this lane's row in the wave's first piece
+  int col;        // its elements of that row
+  int64_t sN;
+  uint32_t off;   // both, in bytes
+  const __bf16* base;
+  __device__ __forceinline__ WaMove(int lane, int wave) {
+    first = wave * R + lane / G;
+    // pieces NW apart have the same swizzle: it looks at a row modulo 16
+    static_assert(NW * R % 16 == 0, "swizzle of a wave's pieces");
+    col = ((lane % G) ^ wa_swz<D>(first)) * 8;
+  }
+  __device__ __forceinline__ void from(const __bf16* p, int64_t rows) {
+    base = p;
+    sN = rows;
+    off = (uint32_t)((first * (uint32_t)rows + col) * 2);
+  }
+  __device__ __forceinline__ void go(int row0, int len, char* lds, int wave) const {
 #pragma unroll
-      for (int i = 0; i < CNT; ++i) {
-        const char* at = (const char*)(base + (row0 + i * STEP) * sN);
-        v[i] = *(const wa_u4*)(at + off);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CNT; ++i) {
-        const int row = min(row0 + (int)r + i * STEP, len - 1);
-        v[i] = *(const wa_u4*)(base + row * sN + g * 8);
-      }
+    for (int i = 0; i < CNT; ++i) {
+      const char* at;
+      if (row0 + WA_T <= len)
+        at = (const char*)(base + (row0 + i * NW * R) * sN) + off;
+      else
+        at = (const char*)(base + min(row0 + first + i * NW * R, len - 1) * sN + col);
+      __builtin_amdgcn_global_load_lds((wa_mem*)at, (wa_lds*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
     }
-  }
-  __device__ __forceinline__ static int place() {  // of v[0], in bytes
-    const int g = threadIdx.x % G, r = threadIdx.x / G;
-    return r * D * 2 + ((g ^ wa_swz<D>(r)) * 16);
-  }
-  // rows STEP apart have the same swizzle: it looks at a row modulo 16
-  __device__ __forceinline__ void store(char* lds, int at) const {
-    static_assert(STEP % 16 == 0, "swizzle of rows STEP apart");
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) *(wa_u4*)(lds + at + i * STEP * D * 2) = v[i];
   }
 };
 
@@ -237,6 +253,12 @@ struct WaPlace {
     return it < nsink ? it : first + it - nsink;
   }
 };
+
+// All waves are here, and what they sent to LDS has arrived.
+__device__ __forceinline__ void wa_sync() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
 
 __device__ __forceinline__ int wa_wave() {  // the same for all lanes: a scalar
   return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -330,91 +352,106 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
   wa_row<D>(a.q.p + w.b * a.q.sB + w.head * a.q.sH + min(row, w.len - 1) * a.q.sN, half, qf);
   const WaRows<D> rows(lane);
   const WaCols<D> cols(lane);
-  const int put = WaStage<D>::place();
-  // K and V take turns in the registers of one tile on its way
-  {
-    WaStage<D> st;
-    st.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
-    st.store(lds, put);
-    st.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
-    st.store(lds + TILE, put);
-  }
+  // LDS: two buffers of K, two of V.  Keys are taken 32 at a time; while the
+  // weights of one strip are computed, the next strip's scores run on the
+  // matrix cores, so K is a strip ahead.
+  char* const ldk = lds;
+  char* const ldv = lds + 2 * TILE;
+  const int wave = wa_wave();
+  WaMove<D, 4> mk(lane, wave), mv(lane, wave);
+  mk.from(kb, a.k.sN);
+  mv.from(vb, a.v.sN);
+  mk.go(w.tile(0) * WA_T, w.len, ldk, wave);
+  mv.go(w.tile(0) * WA_T, w.len, ldv, wave);
+  if (w.count > 1) mk.go(w.tile(1) * WA_T, w.len, ldk + TILE, wave);
   const float c = a.scale * WA_LOG2E;
   float m = -3.0e38f, l = 0.0f;  // l: this half wave's keys
-  auto step = [&](int it, char* mine, char* next) {
-    char* tk = mine;
-    char* tv = mine + TILE;
-    const int k0 = w.tile(it) * WA_T;
-    const bool more = it + 1 < w.count;
-    const int n0 = more ? w.tile(it + 1) * WA_T : 0;
-    __syncthreads();
-    WaStage<D> st;
-    if (more) st.load(kb, a.k.sN, n0, w.len);
-    const int seen = wa_seen(a, w.wrow, k0, WA_T);
-    wa_f16 s[2];
-    if (seen) {
+  auto scores = [&](const char* tk, int sub, wa_f16& to) {
+    to = (wa_f16)(0.0f);
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        wa_bf8 f[D / 16];
+    for (int kk = 0; kk < D / 16; ++kk) to = wa_mfma(rows.get(tk, sub, kk), qf[kk], to);
+  };
+  // scaled first: the products need no quieting before the comparisons
+  auto highest = [&](wa_f16& s) {
+    float top = s[0];
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) f[kk] = rows.get(tk, sub, kk);
-        s[sub] = (wa_f16)(0.0f);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s[sub] = wa_mfma(f[kk], qf[kk], s[sub]);
+    for (int r = 1; r < 15; r += 2) top = fmaxf(fmaxf(top, s[r]), s[r + 1]);
+    return fmaxf(top, s[15]);
+  };
+  // the strip's weights and their product; then the next strip's scores
+  auto strip = [&](wa_f16& s, int seen, int k0, const char* tv, int sub, wa_f16& next,
+                   int seen_next, const char* tk, int sub_next) {
+    float top = -INFINITY;
+    if (seen == 2 && seen_next) {
+      scores(tk, sub_next, next);
+      s *= c;
+      top = highest(s);
+      wa_mix<D / 16, D / 16, 4, 1, 3>();
+    } else {
+      if (seen_next) {
+        scores(tk, sub_next, next);
+        wa_feed<D / 16, D / 16, 4, 1>();
       }
-      wa_feed<D / 8, D / 8, 4, 1>();
-    }
-    if (more) {
-      st.store(next, put);
-      st.load(vb, a.v.sN, n0, w.len);
-    }
-    if (seen) {
-      // scaled first: the products need no quieting before the comparisons
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) s[sub] *= c;
-      if (seen == 1) {
-        const WaVis vis = wa_vis_of(a, row, k0, half);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+      if (seen) {
+        s *= c;
+        if (seen == 1) {
+          const WaVis vis = wa_vis_of(a, row, k0, half);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!wa_vis_key(vis, sub * 32 + 8 * (r / 4) + r % 4)) s[sub][r] = -INFINITY;
-      }
-      float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
-      const float mn = fmaxf(m, wa_other_max(top));
-      // weights may pass 1 by a factor of 2^8 before everything is rescaled
-      if (__any(mn > m + 8.0f)) {
-        const float f = wa_exp2(m - mn);
-        l *= f;
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) acc[t] *= f;
-        m = mn;
-      }
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[sub][r] = wa_exp2(s[sub][r] - m);
-          l += s[sub][r];
+            if (!wa_vis_key(vis, 8 * (r / 4) + r % 4)) s[r] = -INFINITY;
         }
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        wa_bf8 f[D / 32];
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) f[t] = cols.get(tv, ks, t);
-        const wa_bf8 p = wa_operand(s[ks >> 1], ks & 1);
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) acc[t] = wa_mfma(f[t], p, acc[t]);
+        top = highest(s);
       }
-      wa_feed<D / 8, D / 4, 8, 2>();
     }
-    if (more) st.store(next + TILE, put);
+    if (seen == 0) return;
+    const float mn = fmaxf(m, wa_other_max(top));
+    // weights may pass 1 by a factor of 2^8 before everything is rescaled
+    if (__any(mn > m + 8.0f)) {
+      const float f = wa_exp2(m - mn);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) acc[t] *= f;
+      m = mn;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int r = 8 * ks; r < 8 * ks + 8; ++r) {
+        s[r] = wa_exp2(s[r] - m);
+        l += s[r];
+      }
+      const wa_bf8 p = wa_operand(s, ks);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+        acc[t] = wa_mfma(cols.get(tv, sub * 2 + ks, t), p, acc[t]);
+    }
+    wa_feed<D / 16, D / 8, 4, 2>();
+  };
+  wa_sync();
+  wa_f16 s0, s1;
+  int seen0 = wa_seen(a, w.wrow, w.tile(0) * WA_T, 32);
+  if (seen0) {
+    scores(ldk, 0, s0);
+    wa_feed<D / 16, D / 16, 4, 1>();
+  }
+  // o: 0 or TILE, where this tile stands
+  auto step = [&](int it, int o) {
+    const int k0 = w.tile(it) * WA_T;
+    const bool more = it + 1 < w.count, more2 = it + 2 < w.count;
+    const int n0 = more ? w.tile(it + 1) * WA_T : 0;
+    const int seen1 = wa_seen(a, w.wrow, k0 + 32, 32);
+    const int seen2 = more ? wa_seen(a, w.wrow, n0, 32) : 0;
+    if (it) wa_sync();
+    if (more) mv.go(n0, w.len, ldv + (TILE - o), wave);
+    strip(s0, seen0, k0, ldv + o, 0, s1, seen1, ldk + o, 1);
+    wa_sync();  // this tile's keys have been read
+    if (more2) mk.go(w.tile(it + 2) * WA_T, w.len, ldk + o, wave);
+    strip(s1, seen1, k0 + 32, ldv + o, 1, s0, seen2, ldk + (TILE - o), 0);
+    seen0 = seen2;
   };
   for (int it = 0; it < w.count; it += 2) {
-    step(it, lds, lds + 2 * TILE);
-    if (it + 1 < w.count) step(it + 1, lds + 2 * TILE, lds);
+    step(it, 0);
+    if (it + 1 < w.count) step(it + 1, TILE);
   }
   l = wa_other_sum(l);
   const bool in = row < w.len;
@@ -468,14 +505,12 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
   if (in && half == 0) a.delta[stat] = delta;
   const WaRows<D> rows(lane);
   const WaCols<D> cols(lane);
-  const int put = WaStage<D>::place();
-  {
-    WaStage<D> st;
-    st.load(kb, a.k.sN, w.tile(0) * WA_T, w.len);
-    st.store(lds, put);
-    st.load(vb, a.v.sN, w.tile(0) * WA_T, w.len);
-    st.store(lds + TILE, put);
-  }
+  const int wave = wa_wave();
+  WaMove<D, 4> mk(lane, wave), mv(lane, wave);
+  mk.from(kb, a.k.sN);
+  mv.from(vb, a.v.sN);
+  mk.go(w.tile(0) * WA_T, w.len, lds, wave);
+  mv.go(w.tile(0) * WA_T, w.len, lds + TILE, wave);
   const float c = a.scale * WA_LOG2E;
   auto step = [&](int it, char* mine, char* next) {
     char* tk = mine;
@@ -483,22 +518,25 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
     const int k0 = w.tile(it) * WA_T;
     const bool more = it + 1 < w.count;
     const int n0 = more ? w.tile(it + 1) * WA_T : 0;
-    __syncthreads();
+    wa_sync();
+    if (more) {
+      mk.go(n0, w.len, next, wave);
+      mv.go(n0, w.len, next + TILE, wave);
+    }
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      WaStage<D> st;
-      if (more) st.load(sub ? vb : kb, sub ? a.v.sN : a.k.sN, n0, w.len);
       const int seen = wa_seen(a, w.wrow, k0 + sub * 32, 32);
       if (seen) {
         wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          s = wa_mfma(rows.get(tk, sub, kk), qf[kk], s);
-          p = wa_mfma(rows.get(tv, sub, kk), gf[kk], p);
-        }
-        wa_feed<D / 8, D / 8, 4, 1>();
+        for (int kk = 0; kk < D / 16; ++kk) s = wa_mfma(rows.get(tk, sub, kk), qf[kk], s);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) p = wa_mfma(rows.get(tv, sub, kk), gf[kk], p);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = wa_exp2(fmaf(s[r], c, -lse));
+        // the exponentials run beside dP's products
+        wa_feed<D / 16, D / 16, 4, 1>();
+        wa_mix<D / 16, D / 16, 4, 1, 4>();
         if (seen == 1) {
           const WaVis vis = wa_vis_of(a, row, k0 + sub * 32, half);
 #pragma unroll
@@ -518,7 +556,6 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
         }
         wa_feed<D / 16, D / 8, 4, 2>();
       }
-      if (more) st.store(next + sub * TILE, put);
     }
   };
   for (int it = 0; it < w.count; it += 2) {
@@ -601,48 +638,50 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
     const int own = part * 32 * D * 2, far = (part ^ (PARTS - 1)) * 32 * D * 2;
     const WaRows<D> rows(lane, own);
     const WaCols<D, DT> cols(lane, part * DT, own), others(lane, part * DT, far);
-    using Stage = WaStage<D, NT>;
-    const int put = Stage::place();
+    WaMove<D, NT / 64> mq(lane, wave), mg(lane, wave);
     char* give = lds + 2 * BUF + wave * 4096 + lane * 16;
     char* take = lds + 2 * BUF + (wave ^ 4) * 4096 + lane * 16;
-    Stage sq, sg;
     float sl = 0.0f, sd = 0.0f;
     const float c = a.scale * WA_LOG2E;
     const bool sinkkey = key < a.sinks;
-    int head = kv * G, tile = 0;  // what is loaded next
-    auto load = [&]() {
+    int head = kv * G, tile = 0;  // what travels next
+    auto load = [&](char* to) {
       const int r0 = (t0 + tile) * WA_T;
-      sq.load(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN, r0, len);
-      sg.load(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN, r0, len);
+      if (tile == 0) {
+        mq.from(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN);
+        mg.from(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN);
+      }
+      mq.go(r0, len, to, wave);
+      mg.go(r0, len, to + TILE, wave);
       if (threadIdx.x < WA_T) {
         const int r = r0 + threadIdx.x;
         const int64_t i = ((int64_t)b * a.H + head) * a.N + min(r, len - 1);
         sl = r < len ? a.lse[i] : INFINITY;  // no weight for rows that are not
         sd = a.delta[i];
       }
+      if (++tile == total) {
+        tile = 0;
+        ++head;
+      }
     };
-    load();
-    int row0 = (t0 + tile) * WA_T;  // of the tile that is stored next
-    auto step = [&](int it, char* buf) {
+    auto keep = [&](char* to) {  // the rows' statistics
+      if (threadIdx.x < WA_T) {
+        ((float*)(to + 2 * TILE))[threadIdx.x] = sl;
+        ((float*)(to + 2 * TILE))[WA_T + threadIdx.x] = sd;
+      }
+    };
+    load(lds);
+    keep(lds);
+    int at_tile = 0;
+    auto step = [&](int it, char* buf, char* next) {
       char* tq = buf;
       char* tg = buf + TILE;
       float* stat = (float*)(buf + 2 * TILE);
-      const int r0 = row0;
-      sq.store(tq, put);
-      sg.store(tg, put);
-      if (threadIdx.x < WA_T) {
-        stat[threadIdx.x] = sl;
-        stat[WA_T + threadIdx.x] = sd;
-      }
-      if (it + 1 < it1) {
-        if (++tile == total) {
-          tile = 0;
-          ++head;
-        }
-        row0 = (t0 + tile) * WA_T;
-        load();
-      }
-      __syncthreads();
+      const int r0 = (t0 + at_tile) * WA_T;
+      if (++at_tile == total) at_tile = 0;
+      const bool more = it + 1 < it1;
+      wa_sync();
+      if (more) load(next);
       auto sum = [&](const WaCols<D, DT>& from, int ks, wa_bf8 pf, wa_bf8 df) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -660,6 +699,9 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           s = wa_mfma(rows.get(tq, in, kk), kf[kk], s);
+        }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
           p = wa_mfma(rows.get(tg, in, kk), vf[kk], p);
         }
         wa_feed<D / 8, D / 8, 4, 1>();
@@ -693,7 +735,7 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
         wa_feed<4 * DT, 8 * DT, 4, 2>();
       }
       if (PARTS == 2) {
-        __syncthreads();
+        wa_sync();
         if (wa_seen(a, r0 + (part ^ 1) * 32, wk, 32)) {
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
@@ -702,10 +744,11 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
           wa_feed<4 * DT, 8 * DT + 4, 8, 2>();
         }
       }
+      if (more) keep(next);
     };
     for (int it = 0; it < it1; it += 2) {
-      step(it, lds);
-      if (it + 1 < it1) step(it + 1, lds + BUF);
+      step(it, lds, lds + BUF);
+      if (it + 1 < it1) step(it + 1, lds + BUF, lds);
     }
   }
   const bool split = a.slots > 0 && key < a.sinks;

@@ -85,63 +85,6 @@ def _join_plain(x, u, w, b, gate, pw, pb, scale, eps, kind):
     return y.to(x.dtype), _norm_plain(y, w, b, kind, eps).to(x.dtype)
 
 
-class _GatedResidual(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, u, w, b, gate, pw, pb, scale, eps, kind, groups,
-                gate_kind):
-        D = x.shape[-1]
-        rows = x.numel() // D // groups
-        x, u, w, b, gate, pw, pb = (
-            None if t is None else t.contiguous()
-            for t in (x, u, w, b, gate, pw, pb))
-        y, h = torch.empty_like(x), torch.empty_like(x)
-        stats = torch.empty(4 if pw is not None else 2, groups * rows,
-                            dtype=torch.float32, device=x.device)
-        layer = kind == "layer"
-        step = D if gate_kind == 1 and groups > 1 else 0
-        _EXT.join_fwd([x, u, w, b, pw, pb, gate, y, h], stats, groups, rows, D,
-                      layer, gate_kind, step, scale, eps)
-        ctx.save_for_backward(y, u, w, gate, pw, pb, stats)
-        ctx.b_dtype = None if b is None else b.dtype
-        ctx.cfg = (groups, rows, D, layer, gate_kind, step, scale)
-        ctx.set_materialize_grads(False)
-        return y, h
-
-    @staticmethod
-    def backward(ctx, dy, dh):
-        y, u, w, gate, pw, pb, stats = ctx.saved_tensors
-        groups, rows, D, layer, gate_kind, step, scale = ctx.cfg
-        need = dict(zip(("x", "u", "w", "b", "gate", "pw", "pb"),
-                        ctx.needs_input_grad))
-        dy, dh = (None if t is None else t.contiguous() for t in (dy, dh))
-        dx, du = torch.empty_like(y), torch.empty_like(u)
-
-        def like(t, wanted):
-            return torch.empty_like(t) if wanted and t is not None else None
-
-        # without dh the last norm's parameters get no gradient
-        dw = like(w, need["w"] and dh is not None)
-        db = None
-        if need["b"] and ctx.b_dtype is not None and dh is not None:
-            db = torch.empty_like(w)
-        dgate = like(gate, need["gate"])
-        dpw, dpb = like(pw, need["pw"]), like(pb, need["pb"])
-        whole = gate_kind == 2
-        sums = [dw, db, None if whole else dgate, dpw, dpb]
-        if dy is not None or dh is not None:
-            nsum = sum(t is not None for t in sums)
-            part = torch.empty(
-                groups * _EXT.join_blocks(groups, rows, D) * nsum * D,
-                dtype=torch.float32, device=y.device)
-            _EXT.join_bwd([u, w, pw, pb, gate, y, dy, dh, dx, du,
-                           dgate if whole else None], stats, sums, part,
-                          groups, rows, D, layer, gate_kind, step, scale)
-        else:
-            return (None,) * 12
-        return (dx if need["x"] else None, du if need["u"] else None, dw, db,
-                dgate, dpw, dpb, None, None, None, None, None)
-
-
 def fused_gated_residual(x, u, weight, bias=None, *, gate=None,
                          post_weight=None, post_bias=None, scale=1.0,
                          eps=1e-5, kind="layer"):
@@ -196,8 +139,8 @@ def fused_gated_residual(x, u, weight, bias=None, *, gate=None,
         if D > MAX_JOIN_DIM:
             raise ValueError(f"fused_gated_residual on GPU: rows of at most "
                              f"{MAX_JOIN_DIM}, got {D}")
-        return _GatedResidual.apply(x, u, weight, bias, gate, post_weight,
-                                    post_bias, float(scale), float(eps), kind,
-                                    groups, gate_kind)
+        return tuple(_EXT.gated_residual(
+            x, u, weight, bias, gate, post_weight, post_bias, float(scale),
+            float(eps), kind == "layer", groups, gate_kind))
     return _join_plain(x, u, weight, bias, gate, post_weight, post_bias,
                        scale, eps, kind)

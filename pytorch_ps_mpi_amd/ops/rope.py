@@ -36,19 +36,6 @@ def _rotate_plain(x, cos, sin, interleaved):
     return torch.cat([y, rest], -1).to(x.dtype)
 
 
-class _Rope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, rot):
-        ctx.save_for_backward(positions)
-        ctx.rot = rot
-        return rot._launch(q, k, positions, False)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        (positions,) = ctx.saved_tensors
-        return (*ctx.rot._launch(dq, dk, positions, True), None, None)
-
-
 class AxialRotary:
     """Rotary embedding of q and k by positions on several axes.
 
@@ -113,7 +100,8 @@ class AxialRotary:
     def __call__(self, q, k, positions):
         positions = self._check(q, k, positions)
         if _require_ext(q):
-            return _Rope.apply(q, k, positions, self)
+            return tuple(_EXT.rope(q, k, positions, self._start, self._rev,
+                                   self.interleaved))
         cos, sin = self._angles(positions)
         return (_rotate_plain(q, cos, sin, self.interleaved),
                 _rotate_plain(k, cos, sin, self.interleaved))
@@ -124,11 +112,3 @@ class AxialRotary:
         t = positions.double()[axis].permute(1, 2, 0) * self.freq
         return torch.cos(t).float()[:, :, None], \
             torch.sin(t).float()[:, :, None]
-
-    def _launch(self, q, k, positions, backward):
-        q, k = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k))
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _EXT.rope(q, k, yq, yk, positions, self._start, self._rev,
-                  self.interleaved, backward)
-        return yq, yk

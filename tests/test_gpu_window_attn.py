@@ -228,5 +228,8 @@ def test_types_without_kernel_and_refusals():
         fused_window_sdpa(q, k, v, 9, lengths=torch.tensor([3],
                                                            dtype=torch.int32))
     with pytest.raises(RuntimeError):  # the extension checks for itself
-        attn._EXT.wa_fwd(q, k, v, q, torch.zeros(80, device=DEV), None, 9, 0,
-                         1.0)
+        attn._EXT.window_sdpa(q, k, v[:, :, :9], 9, 0, None, 1.0)
+    x = q.detach().requires_grad_()
+    o = fused_window_sdpa(x, k, v, 9)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(o.sum(), x, create_graph=True)
