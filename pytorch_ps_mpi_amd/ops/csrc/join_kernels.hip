@@ -56,12 +56,12 @@ struct JnRow {
   __device__ __forceinline__ static int at(int j, int lane) {
     return ((j / VEC) * TPR + lane) * VEC + j % VEC;
   }
-  // past the row's end: zeros
+  // past the row's end, and where there is no tensor: zeros
   __device__ __forceinline__ void load(const void* p, int64_t off, int lane, int D) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e = (i * TPR + lane) * VEC;
-      if (e < D) {
+      if (p != nullptr && e < D) {
         c[i] = *(const JnVec<T, VEC>*)((const T*)p + off + e);
       } else {
 #pragma unroll
@@ -80,14 +80,28 @@ struct JnRow {
   __device__ __forceinline__ void set(int j, float v) { c[j / VEC].v[j % VEC] = jn_t<T>(v); }
 };
 
+// The sum over a wave, in all lanes, without LDS: rotations within 16 lanes,
+// then rows of 16 and halves swapped.  All lanes add the same pairs: one value.
+__device__ __forceinline__ float jn_wave_sum(float x) {
+#define JN_ROR(n)                                                              \
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(                            \
+      0, __float_as_uint(x), 0x120 + (n), 0xf, 0xf, false))
+  JN_ROR(8);
+  JN_ROR(4);
+  JN_ROR(2);
+  JN_ROR(1);
+#undef JN_ROR
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // Sums over the lanes of a row.  `red`: room for two rounds of a block's waves.
 template <int TPR>
 __device__ __forceinline__ float2 jn_sum2(float a, float b, float2* red, int& turn) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    a += __shfl_xor(a, d, 64);
-    b += __shfl_xor(b, d, 64);
-  }
+  a = jn_wave_sum(a);
+  b = jn_wave_sum(b);
   if (TPR == 64) return make_float2(a, b);
   constexpr int W = TPR / 64;
   float2* r = red + turn * W;
@@ -129,11 +143,17 @@ __device__ __forceinline__ void jn_stats(const JoinArgs& a, const float* f, int 
   rstd = 1.0f / sqrtf(fmaf(q, a.invD, a.eps));
 }
 
-template <typename T, int VEC, int EPT, int TPR, bool POST>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
-k_join_fwd(const JoinArgs a) {
+// Rows of 64 lanes stand four to a block, others are a block each.
+template <int TPR>
+struct JnBlock {
+  static constexpr int N = TPR < 128 ? 256 : TPR, ROWS = N / TPR;
+};
+
+// GATE: 0 none, 1 a vector, 2 x's shape
+template <typename T, int VEC, int EPT, int TPR, bool POST, int GATE>
+__global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_fwd(const JoinArgs a) {
   using R = JnRow<T, VEC, EPT, TPR>;
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;  // rows a block has in hand
+  constexpr int RPB = JnBlock<TPR>::ROWS;
   __shared__ float2 red[2 * (TPR / 64)];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int group = blockIdx.x / a.nb, blk = blockIdx.x - group * a.nb;
@@ -141,18 +161,27 @@ k_join_fwd(const JoinArgs a) {
   int turn = 0;
   R w, b, pw, pb, gate;
   w.load(a.w, 0, lane, D);
-  if (a.b) b.load(a.b, 0, lane, D);
+  b.load(a.b, 0, lane, D);
   if (POST) {
     pw.load(a.pw, 0, lane, D);
-    if (a.pb) pb.load(a.pb, 0, lane, D);
+    pb.load(a.pb, 0, lane, D);
   }
-  if (a.gate_kind == 1) gate.load(a.gate, group * a.gate_step, lane, D);
-  for (int64_t i = (int64_t)blk * RPB + sub; i < a.rows; i += (int64_t)a.nb * RPB) {
+  if (GATE == 1) gate.load(a.gate, group * a.gate_step, lane, D);
+  const int64_t step = (int64_t)a.nb * RPB;
+  int64_t i = (int64_t)blk * RPB + sub;
+  R xn, un, gn;  // the next row's, on their way
+  auto load = [&](int64_t at) {
+    const int64_t off = (group * a.rows + at) * D;
+    xn.load(a.x, off, lane, D);
+    un.load(a.u, off, lane, D);
+    if (GATE == 2) gn.load(a.gate, off, lane, D);
+  };
+  if (i < a.rows) load(i);
+  for (; i < a.rows; i += step) {
     const int64_t row = group * a.rows + i, off = row * D;
-    R x, u;
-    x.load(a.x, off, lane, D);
-    u.load(a.u, off, lane, D);
-    if (a.gate_kind == 2) gate.load(a.gate, off, lane, D);
+    R x = xn, u = un;
+    if (GATE == 2) gate = gn;
+    if (i + step < a.rows) load(i + step);
     float f[EPT];
 #pragma unroll
     for (int j = 0; j < EPT; ++j) f[j] = u.get(j);
@@ -164,12 +193,11 @@ k_join_fwd(const JoinArgs a) {
         a.ru[row] = r;
       }
 #pragma unroll
-      for (int j = 0; j < EPT; ++j)
-        f[j] = fmaf((f[j] - m) * r, pw.get(j), a.pb ? pb.get(j) : 0.0f);
+      for (int j = 0; j < EPT; ++j) f[j] = fmaf((f[j] - m) * r, pw.get(j), pb.get(j));
     }
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
-      const float g = a.gate_kind ? gate.get(j) * f[j] : f[j];
+      const float g = GATE ? gate.get(j) * f[j] : f[j];
       f[j] = R::at(j, lane) < D ? fmaf(a.scale, x.get(j), g) : 0.0f;
       x.set(j, f[j]);
     }
@@ -181,18 +209,17 @@ k_join_fwd(const JoinArgs a) {
       a.ry[row] = r;
     }
 #pragma unroll
-    for (int j = 0; j < EPT; ++j)
-      u.set(j, fmaf((f[j] - m) * r, w.get(j), a.b ? b.get(j) : 0.0f));
+    for (int j = 0; j < EPT; ++j) u.set(j, fmaf((f[j] - m) * r, w.get(j), b.get(j)));
     u.store(a.h, off, lane, D);
   }
 }
 
-// This block's sums of one slot, to its part: the RPB rows in hand are added
+// This block's sums of one slot, to its part: the rows in hand are added
 // through LDS in fixed order.
 template <int VEC, int EPT, int TPR, typename R>
 __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int slot,
                                         int lane, int sub, float* lds) {
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  constexpr int RPB = JnBlock<TPR>::ROWS;
   if (slot < 0) return;
   float* out = a.part + ((int64_t)blockIdx.x * a.slots + slot) * a.D;
   if (RPB == 1) {
@@ -205,7 +232,7 @@ __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int
 #pragma unroll
   for (int j = 0; j < EPT; ++j) lds[sub * EPT * TPR + R::at(j, lane)] = acc[j];
   __syncthreads();
-  for (int e = threadIdx.x; e < a.D; e += 256) {
+  for (int e = threadIdx.x; e < a.D; e += JnBlock<TPR>::N) {
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < RPB; ++k) s += lds[k * EPT * TPR + e];
@@ -213,11 +240,10 @@ __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int
   }
 }
 
-template <typename T, int VEC, int EPT, int TPR, bool POST>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
-k_join_bwd(const JoinArgs a) {
+template <typename T, int VEC, int EPT, int TPR, bool POST, int GATE>
+__global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) {
   using R = JnRow<T, VEC, EPT, TPR>;
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  constexpr int RPB = JnBlock<TPR>::ROWS;
   __shared__ float2 red[2 * (TPR / 64)];
   __shared__ float lds[RPB == 1 ? 1 : RPB * EPT * TPR];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -225,69 +251,71 @@ k_join_bwd(const JoinArgs a) {
   const int D = a.D;
   int turn = 0;
   R w, pw, pb, gate;
-  float aw[EPT], ab[EPT], ag[EPT], apw[POST ? EPT : 1], apb[POST ? EPT : 1];
+  float aw[EPT], ab[EPT], ag[GATE == 1 ? EPT : 1], apw[POST ? EPT : 1], apb[POST ? EPT : 1];
 #pragma unroll
   for (int j = 0; j < EPT; ++j) {
-    aw[j] = ab[j] = ag[j] = 0.0f;
+    aw[j] = ab[j] = 0.0f;
+    if (GATE == 1) ag[j] = 0.0f;
     if (POST) apw[j] = apb[j] = 0.0f;
   }
   w.load(a.w, 0, lane, D);
   if (POST) {
     pw.load(a.pw, 0, lane, D);
-    if (a.pb) pb.load(a.pb, 0, lane, D);
+    if (GATE) pb.load(a.pb, 0, lane, D);
   }
-  if (a.gate_kind == 1) gate.load(a.gate, group * a.gate_step, lane, D);
-  for (int64_t i = (int64_t)blk * RPB + sub; i < a.rows; i += (int64_t)a.nb * RPB) {
-    const int64_t row = group * a.rows + i, off = row * D;
-    R y, u, dy, dh;
-    if (a.dh) {
-      y.load(a.y, off, lane, D);
-      dh.load(a.dh, off, lane, D);
-    }
-    u.load(a.u, off, lane, D);
-    if (a.dy) dy.load(a.dy, off, lane, D);
-    if (a.gate_kind == 2) gate.load(a.gate, off, lane, D);
-    float t[EPT];  // the whole gradient of y
-    if (a.dh) {
-      const float m = a.my[row], r = a.ry[row];
-      float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-      for (int j = 0; j < EPT; ++j) {
-        const float xh = (y.get(j) - m) * r, g = dh.get(j);
-        aw[j] = fmaf(g, xh, aw[j]);
-        ab[j] += g;
-        const float k = g * w.get(j);
-        s1 += k;
-        s2 = fmaf(k, xh, s2);
-      }
-      const float2 s = jn_sum2<TPR>(s1, s2, red, turn);
-      const float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
-#pragma unroll
-      for (int j = 0; j < EPT; ++j) {
-        const float xh = (y.get(j) - m) * r;
-        t[j] = r * (fmaf(dh.get(j), w.get(j), -c1) - xh * c2);
-        if (a.dy) t[j] += dy.get(j);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPT; ++j) t[j] = a.dy ? dy.get(j) : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < EPT; ++j) y.set(j, a.scale * t[j]);
-    y.store(a.dx, off, lane, D);
-    float m = 0.0f, r = 1.0f, s1 = 0.0f, s2 = 0.0f;
+  if (GATE == 1) gate.load(a.gate, group * a.gate_step, lane, D);
+  const int64_t step = (int64_t)a.nb * RPB;
+  int64_t i = (int64_t)blk * RPB + sub;
+  R yn, un, dyn, dhn, gn;  // the next row's, on their way
+  float m1n = 0.0f, r1n = 0.0f, m2n = 0.0f, r2n = 1.0f;
+  auto load = [&](int64_t at) {
+    const int64_t row = group * a.rows + at, off = row * D;
+    m1n = a.my[row];
+    r1n = a.ry[row];
     if (POST) {
-      m = a.mu[row];
-      r = a.ru[row];
+      m2n = a.mu[row];
+      r2n = a.ru[row];
     }
+    yn.load(a.y, off, lane, D);
+    dhn.load(a.dh, off, lane, D);
+    dyn.load(a.dy, off, lane, D);
+    un.load(a.u, off, lane, D);
+    if (GATE == 2) gn.load(a.gate, off, lane, D);
+  };
+  if (i < a.rows) load(i);
+  for (; i < a.rows; i += step) {
+    const int64_t row = group * a.rows + i, off = row * D;
+    R y = yn, u = un, dy = dyn, dh = dhn;
+    if (GATE == 2) gate = gn;
+    const float m1 = m1n, r1 = r1n, m2 = m2n, r2 = r2n;
+    if (i + step < a.rows) load(i + step);
+    float t[EPT];  // the whole gradient of y
+    float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
-      const float uh = POST ? (u.get(j) - m) * r : u.get(j);
-      if (a.gate_kind) {
-        const float n = POST ? fmaf(uh, pw.get(j), a.pb ? pb.get(j) : 0.0f) : uh;
-        const float g = t[j] * n;
-        ag[j] += g;
-        dy.set(j, g);
+      const float xh = (y.get(j) - m1) * r1, g = dh.get(j);
+      aw[j] = fmaf(g, xh, aw[j]);
+      ab[j] += g;
+      t[j] = g * w.get(j);
+      s1 += t[j];
+      s2 = fmaf(t[j], xh, s2);
+    }
+    float2 s = jn_sum2<TPR>(s1, s2, red, turn);
+    float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD * r1;
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) {
+      t[j] = fmaf(r1, fmaf(m1 - y.get(j), c2, t[j] - c1), dy.get(j));
+      y.set(j, a.scale * t[j]);
+    }
+    y.store(a.dx, off, lane, D);
+    s1 = s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) {
+      const float uh = POST ? (u.get(j) - m2) * r2 : u.get(j);
+      if (GATE) {
+        const float g = t[j] * (POST ? fmaf(uh, pw.get(j), pb.get(j)) : uh);
+        if (GATE == 1) ag[j] += g;
+        if (GATE == 2) dy.set(j, g);
         t[j] *= gate.get(j);
       }
       if (POST) {
@@ -298,13 +326,13 @@ k_join_bwd(const JoinArgs a) {
         s2 = fmaf(t[j], uh, s2);
       }
     }
-    if (a.dgate) dy.store(a.dgate, off, lane, D);
+    if (GATE == 2 && a.dgate) dy.store(a.dgate, off, lane, D);
     if (POST) {
-      const float2 s = jn_sum2<TPR>(s1, s2, red, turn);
-      const float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
+      s = jn_sum2<TPR>(s1, s2, red, turn);
+      c1 = a.layer ? s.x * a.invD : 0.0f;
+      c2 = s.y * a.invD * r2;
 #pragma unroll
-      for (int j = 0; j < EPT; ++j)
-        t[j] = r * (t[j] - c1 - (u.get(j) - m) * r * c2);
+      for (int j = 0; j < EPT; ++j) t[j] = r2 * fmaf(m2 - u.get(j), c2, t[j] - c1);
     }
 #pragma unroll
     for (int j = 0; j < EPT; ++j) u.set(j, t[j]);
@@ -313,7 +341,7 @@ k_join_bwd(const JoinArgs a) {
   // lanes past the row's end held w = pw = 0 and are not written
   jn_part<VEC, EPT, TPR, R>(a, aw, a.slot_w, lane, sub, lds);
   jn_part<VEC, EPT, TPR, R>(a, ab, a.slot_b, lane, sub, lds);
-  jn_part<VEC, EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
+  if (GATE == 1) jn_part<VEC, EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
   if (POST) {
     jn_part<VEC, EPT, TPR, R>(a, apw, a.slot_pw, lane, sub, lds);
     jn_part<VEC, EPT, TPR, R>(a, apb, a.slot_pb, lane, sub, lds);
@@ -327,12 +355,12 @@ struct JoinSums {
 };
 
 // out[slot][d] = sum over blocks of part[block][slot][d]; the gate's slot one
-// sum for each group.  64 columns and 16 ranges of blocks a thread block.
+// sum for each group.  32 columns and 32 ranges of blocks a thread block.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
-  __shared__ float lds[16][64];
-  const int col = threadIdx.x & 63, rg = threadIdx.x >> 6;
-  const int d = blockIdx.x * 64 + col;
+  __shared__ float lds[32][33];
+  const int col = threadIdx.x & 31, rg = threadIdx.x >> 5;
+  const int d = blockIdx.x * 32 + col;
   // y: first the slots summed over all blocks, then the gate's groups
   const bool each = a.slot_g >= 0 && a.groups > 1;
   const int whole = a.slots - (each ? 1 : 0);
@@ -349,63 +377,96 @@ __global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
     count = a.nb;
   }
   float s = 0.0f;
-  if (d < a.D)
-    for (int i = rg; i < count; i += 16)
-      s += a.part[((int64_t)(first + i) * a.slots + slot) * a.D + d];
+  if (d < a.D) {
+    const float* p = a.part + ((int64_t)first * a.slots + slot) * a.D + d;
+    const int64_t step = (int64_t)a.slots * a.D;
+#pragma unroll 8
+    for (int i = rg; i < count; i += 32) s += p[i * step];
+  }
   lds[rg][col] = s;
   __syncthreads();
-  if (rg == 0 && d < a.D) {
+  // the ranges of a column in one half wave
+  s = lds[col][rg];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += lds[i][col];
-    ((T*)a.out[slot])[(int64_t)g * a.D + d] = jn_t<T>(s);
-  }
+  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor(s, k, 32);
+  const int e = blockIdx.x * 32 + rg;
+  if (col == 0 && e < a.D) ((T*)a.out[slot])[(int64_t)g * a.D + e] = jn_t<T>(s);
 }
 
 // ---------------------------------------------------------------------------
 
-static inline int jn_rpb(int D) { return D <= 1024 ? 4 : 1; }
+// Lanes and elements a lane for a row of D.  Eight elements a lane keep the
+// backward kernel with Post at two waves a SIMD (16 took 256 registers and left
+// one); without Post 16 fit.  768 = 64 lanes of 12 without idle lanes.
+struct JnShape {
+  int ept, tpr;
+};
+static constexpr JnShape jn_shape(int64_t D, bool lean) {
+  if (D <= 512) return {8, 64};
+  if (D <= 768) return {12, 64};
+  if (D <= 1024) return lean ? JnShape{8, 128} : JnShape{16, 64};
+  if (D <= 2048) return {8, 256};
+  if (D <= 4096) return lean ? JnShape{8, 512} : JnShape{16, 256};
+  return {16, 512};
+}
 
-template <typename T, int VEC, bool BWD, bool POST>
+// DMAX: the longest row of the shape
+template <typename T, int VEC, bool BWD, bool POST, int GATE, int DMAX>
+static void jn_go(hipStream_t s, int grid, const JoinArgs& a) {
+  constexpr JnShape h = jn_shape(DMAX, BWD && POST);
+  constexpr int V = h.ept % VEC == 0 ? VEC : 4, N = JnBlock<h.tpr>::N;
+  if constexpr (BWD)
+    hipLaunchKernelGGL((k_join_bwd<T, V, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_join_fwd<T, V, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
+}
+
+template <typename T, int VEC, bool BWD, bool POST, int GATE>
 static void jn_launch(hipStream_t s, int grid, const JoinArgs& a) {
-#define JN_GO(EPT, TPR)                                                        \
-  do {                                                                         \
-    if (BWD)                                                                   \
-      hipLaunchKernelGGL((k_join_bwd<T, VEC, EPT, TPR, POST>), dim3(grid),     \
-                         dim3(TPR < 256 ? 256 : TPR), 0, s, a);                \
-    else                                                                       \
-      hipLaunchKernelGGL((k_join_fwd<T, VEC, EPT, TPR, POST>), dim3(grid),     \
-                         dim3(TPR < 256 ? 256 : TPR), 0, s, a);                \
-  } while (0)
-  if (a.D <= 512) JN_GO(8, 64);
-  else if (a.D <= 1024) JN_GO(16, 64);
-  else if (a.D <= 2048) JN_GO(8, 256);
-  else if (a.D <= 4096) JN_GO(16, 256);
-  else JN_GO(16, 512);
-#undef JN_GO
+  if (a.D <= 512) jn_go<T, VEC, BWD, POST, GATE, 512>(s, grid, a);
+  else if (a.D <= 768) jn_go<T, VEC, BWD, POST, GATE, 768>(s, grid, a);
+  else if (a.D <= 1024) jn_go<T, VEC, BWD, POST, GATE, 1024>(s, grid, a);
+  else if (a.D <= 2048) jn_go<T, VEC, BWD, POST, GATE, 2048>(s, grid, a);
+  else if (a.D <= 4096) jn_go<T, VEC, BWD, POST, GATE, 4096>(s, grid, a);
+  else jn_go<T, VEC, BWD, POST, GATE, JN_MAXD>(s, grid, a);
+}
+
+template <typename T, int VEC, bool BWD>
+static void jn_form(hipStream_t s, int grid, const JoinArgs& a) {
+  const bool post = a.pw != nullptr;
+  if (post && a.gate_kind == 2) jn_launch<T, VEC, BWD, true, 2>(s, grid, a);
+  else if (post && a.gate_kind == 1) jn_launch<T, VEC, BWD, true, 1>(s, grid, a);
+  else if (post) jn_launch<T, VEC, BWD, true, 0>(s, grid, a);
+  else if (a.gate_kind == 2) jn_launch<T, VEC, BWD, false, 2>(s, grid, a);
+  else if (a.gate_kind == 1) jn_launch<T, VEC, BWD, false, 1>(s, grid, a);
+  else jn_launch<T, VEC, BWD, false, 0>(s, grid, a);
 }
 
 template <typename T, bool BWD>
 static void jn_pick(hipStream_t s, int grid, const JoinArgs& a, bool vec) {
-  constexpr int V = 16 / sizeof(T);
-  const bool post = a.pw != nullptr;
-  if (vec && post) jn_launch<T, V, BWD, true>(s, grid, a);
-  else if (vec) jn_launch<T, V, BWD, false>(s, grid, a);
-  else if (post) jn_launch<T, 1, BWD, true>(s, grid, a);
-  else jn_launch<T, 1, BWD, false>(s, grid, a);
+  if (vec) jn_form<T, 16 / sizeof(T), BWD>(s, grid, a);
+  else jn_form<T, 1, BWD>(s, grid, a);
 }
 
-// Blocks of a group: the backward kernel's registers let 512 blocks be on the
+// Blocks of a group: the backward kernel's registers let 2048 waves be on the
 // chip at once; more would only write more parts.
-extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D,
-                                  int backward) {
-  const int64_t most = (backward ? 512 : 2048) / groups;
-  int64_t nb = (rows + jn_rpb((int)D) - 1) / jn_rpb((int)D);
+static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool post, bool backward) {
+  const JnShape h = jn_shape(D, post && backward);
+  const int64_t rpb = h.tpr < 128 ? 256 / h.tpr : 1;
+  const int64_t waves = h.tpr < 128 ? 4 : h.tpr / 64;
+  const int64_t most = (backward ? 2048 : 8192) / waves / groups;
+  int64_t nb = (rows + rpb - 1) / rpb;
   if (nb > most) nb = most;
   return nb < 1 ? 1 : nb;
 }
 
+extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post) {
+  return jn_blocks(groups, rows, D, post != 0, true);
+}
+
 static int jn_check(const JoinArgs& a, int64_t groups) {
-  if (a.D < 1 || a.D > JN_MAXD || groups * a.nb > 0x7fffffff) return 9003;
+  if (a.D < 1 || a.D > JN_MAXD || groups > 65530 || groups * a.nb > 0x7fffffff)
+    return 9003;
   return 0;
 }
 
@@ -427,7 +488,7 @@ extern "C" int ps_join_fwd(void* stream, void* const* t, float* const* stats,
   a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
   a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
   a.gate_step = gate_step; a.scale = scale; a.eps = eps; a.invD = 1.0f / (float)D;
-  a.nb = (int)ps_join_blocks(groups, rows, D, 0);
+  a.nb = (int)jn_blocks(groups, rows, D, a.pw != nullptr, false);
   if (int e = jn_check(a, groups)) return e;
   const bool vec = jn_vec((const void* const*)t, 9, (int)D, bf16);
   const int grid = (int)(groups * a.nb);
@@ -450,7 +511,7 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
   a.part = part;
   a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
   a.gate_step = gate_step; a.scale = scale; a.invD = 1.0f / (float)D;
-  a.nb = (int)ps_join_blocks(groups, rows, D, 1);
+  a.nb = (int)jn_blocks(groups, rows, D, a.pw != nullptr, true);
   if (int e = jn_check(a, groups)) return e;
   JoinSums q{};
   int* slot[5] = {&a.slot_w, &a.slot_b, &a.slot_g, &a.slot_pw, &a.slot_pb};
@@ -468,7 +529,7 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
   q.part = part; q.slots = a.slots; q.slot_g = a.slot_g;
   q.groups = (int)groups; q.nb = a.nb; q.D = (int)D;
   const int gy = a.slots + (a.slot_g >= 0 && groups > 1 ? (int)groups - 1 : 0);
-  const dim3 sg((unsigned)((D + 63) / 64), (unsigned)gy);
+  const dim3 sg((unsigned)((D + 31) / 32), (unsigned)gy);
   if (bf16) hipLaunchKernelGGL((k_join_sum<__hip_bfloat16>), sg, dim3(1024), 0, s, q);
   else hipLaunchKernelGGL((k_join_sum<float>), sg, dim3(1024), 0, s, q);
   return (int)hipGetLastError();
