@@ -27,7 +27,8 @@ int ps_rope(void* stream, const void* q, const void* k, void* yq, void* yk,
             const void* pos, int pos64, int dtype, const int64_t* strides,
             int64_t B, int64_t N, int H, int KV, int D, int P,
             const int* start, const double* rev, int inter, int backward);
-int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post);
+int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post,
+                       int bf16);
 int ps_join_fwd(void* stream, void* const* t, float* const* stats, int bf16,
                 int64_t groups, int64_t rows, int64_t D, int layer,
                 int gate_kind, int64_t gate_step, float scale, float eps);
@@ -459,7 +460,8 @@ void join_bwd(OptTensors t, at::Tensor stats, OptTensors sums, at::Tensor part,
   int64_t slots = 0;
   for (void* q : s) slots += q != nullptr;
   TORCH_CHECK(part.numel() >=
-                  groups * ps_join_blocks(groups, rows, D, p[2] != nullptr) * slots * D,
+                  groups * ps_join_blocks(groups, rows, D, p[2] != nullptr,
+                                           is_bf16(u)) * slots * D,
               "join_bwd: part too small");
   const c10::DeviceGuard guard(u.device());
   throw_on(ps_join_bwd(cur_stream(u), p, st, s, part.data_ptr<float>(),
@@ -535,7 +537,8 @@ struct GatedResidual : torch::autograd::Function<GatedResidual> {
     int64_t slots = vec.has_value();
     for (int i : {2, 3, 5, 6}) slots += out[i].defined();
     auto part = at::empty({groups *
-                           ps_join_blocks(groups, rows, D, pw.defined()) *
+                           ps_join_blocks(groups, rows, D, pw.defined(),
+                                          is_bf16(u)) *
                            slots * D},
                           y.options().dtype(at::kFloat));
     join_bwd({u, w, opt(pw), opt(pb), opt(gate), y, dy, dh, out[0], out[1],

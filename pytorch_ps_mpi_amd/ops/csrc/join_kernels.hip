@@ -40,7 +40,10 @@ struct JoinArgs {
   float scale, eps, invD;
 };
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) JnVec { T v[VEC]; };
+// 16 bytes at any address that is a multiple of two: rows of odd length are
+// read as wide as others.
+typedef uint32_t jn_u4 __attribute__((ext_vector_type(4)));
+typedef jn_u4 jn_u4_any __attribute__((aligned(2)));
 
 __device__ __forceinline__ float jn_f(float v) { return v; }
 __device__ __forceinline__ float jn_f(__hip_bfloat16 v) { return __bfloat162float(v); }
@@ -48,11 +51,11 @@ template <typename T> __device__ __forceinline__ T jn_t(float v);
 template <> __device__ __forceinline__ float jn_t(float v) { return v; }
 template <> __device__ __forceinline__ __hip_bfloat16 jn_t(float v) { return __float2bfloat16(v); }
 
-// A lane's share of a row: EPT elements in vectors of VEC, TPR lanes a row.
-template <typename T, int VEC, int EPT, int TPR>
+// A lane's share of a row: EPT elements in 16-byte vectors, TPR lanes a row.
+template <typename T, int EPT, int TPR>
 struct JnRow {
-  static constexpr int CH = EPT / VEC;
-  JnVec<T, VEC> c[CH];
+  static constexpr int VEC = 16 / sizeof(T), CH = EPT / VEC;
+  jn_u4 c[CH];
   __device__ __forceinline__ static int at(int j, int lane) {
     return ((j / VEC) * TPR + lane) * VEC + j % VEC;
   }
@@ -61,11 +64,15 @@ struct JnRow {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e = (i * TPR + lane) * VEC;
-      if (p != nullptr && e < D) {
-        c[i] = *(const JnVec<T, VEC>*)((const T*)p + off + e);
+      const T* from = (const T*)p + off + e;
+      if (p != nullptr && e + VEC <= D) {
+        c[i] = *(const jn_u4_any*)from;
       } else {
+        c[i] = (jn_u4)(0u);
+        if (p != nullptr)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) c[i].v[j] = jn_t<T>(0.0f);
+          for (int j = 0; j < VEC; ++j)
+            if (e + j < D) put(i * VEC + j, from[j]);
       }
     }
   }
@@ -73,11 +80,30 @@ struct JnRow {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e = (i * TPR + lane) * VEC;
-      if (e < D) *(JnVec<T, VEC>*)((T*)p + off + e) = c[i];
+      T* to = (T*)p + off + e;
+      if (e + VEC <= D) {
+        *(jn_u4_any*)to = c[i];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (e + j < D) to[j] = of(i * VEC + j);
+      }
     }
   }
-  __device__ __forceinline__ float get(int j) const { return jn_f(c[j / VEC].v[j % VEC]); }
-  __device__ __forceinline__ void set(int j, float v) { c[j / VEC].v[j % VEC] = jn_t<T>(v); }
+  __device__ __forceinline__ T of(int j) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, (uint32_t)c[j / 4][j % 4]);
+    else return __builtin_bit_cast(T, (uint16_t)(c[j / 8][j % 8 / 2] >> (16 * (j & 1))));
+  }
+  __device__ __forceinline__ void put(int j, T v) {
+    if constexpr (sizeof(T) == 4) {
+      c[j / 4][j % 4] = __builtin_bit_cast(uint32_t, v);
+    } else {
+      const uint32_t b = __builtin_bit_cast(uint16_t, v), w = c[j / 8][j % 8 / 2];
+      c[j / 8][j % 8 / 2] = j & 1 ? (w & 0xffffu) | (b << 16) : (w & 0xffff0000u) | b;
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return jn_f(of(j)); }
+  __device__ __forceinline__ void set(int j, float v) { put(j, jn_t<T>(v)); }
 };
 
 // The sum over a wave, in all lanes, without LDS: rotations within 16 lanes,
@@ -150,9 +176,9 @@ struct JnBlock {
 };
 
 // GATE: 0 none, 1 a vector, 2 x's shape
-template <typename T, int VEC, int EPT, int TPR, bool POST, int GATE>
+template <typename T, int EPT, int TPR, bool POST, int GATE>
 __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_fwd(const JoinArgs a) {
-  using R = JnRow<T, VEC, EPT, TPR>;
+  using R = JnRow<T, EPT, TPR>;
   constexpr int RPB = JnBlock<TPR>::ROWS;
   __shared__ float2 red[2 * (TPR / 64)];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -216,7 +242,7 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_fwd(const JoinArgs a) 
 
 // This block's sums of one slot, to its part: the rows in hand are added
 // through LDS in fixed order.
-template <int VEC, int EPT, int TPR, typename R>
+template <int EPT, int TPR, typename R>
 __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int slot,
                                         int lane, int sub, float* lds) {
   constexpr int RPB = JnBlock<TPR>::ROWS;
@@ -240,9 +266,9 @@ __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int
   }
 }
 
-template <typename T, int VEC, int EPT, int TPR, bool POST, int GATE>
+template <typename T, int EPT, int TPR, bool POST, int GATE>
 __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) {
-  using R = JnRow<T, VEC, EPT, TPR>;
+  using R = JnRow<T, EPT, TPR>;
   constexpr int RPB = JnBlock<TPR>::ROWS;
   __shared__ float2 red[2 * (TPR / 64)];
   __shared__ float lds[RPB == 1 ? 1 : RPB * EPT * TPR];
@@ -282,13 +308,16 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
     un.load(a.u, off, lane, D);
     if (GATE == 2) gn.load(a.gate, off, lane, D);
   };
-  if (i < a.rows) load(i);
+  // the longest rows have no registers to hold another one
+  constexpr bool AHEAD = TPR < 512 || EPT < 16;
+  if (AHEAD && i < a.rows) load(i);
   for (; i < a.rows; i += step) {
     const int64_t row = group * a.rows + i, off = row * D;
+    if (!AHEAD) load(i);
     R y = yn, u = un, dy = dyn, dh = dhn;
     if (GATE == 2) gate = gn;
     const float m1 = m1n, r1 = r1n, m2 = m2n, r2 = r2n;
-    if (i + step < a.rows) load(i + step);
+    if (AHEAD && i + step < a.rows) load(i + step);
     float t[EPT];  // the whole gradient of y
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -339,12 +368,12 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
     u.store(a.du, off, lane, D);
   }
   // lanes past the row's end held w = pw = 0 and are not written
-  jn_part<VEC, EPT, TPR, R>(a, aw, a.slot_w, lane, sub, lds);
-  jn_part<VEC, EPT, TPR, R>(a, ab, a.slot_b, lane, sub, lds);
-  if (GATE == 1) jn_part<VEC, EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
+  jn_part<EPT, TPR, R>(a, aw, a.slot_w, lane, sub, lds);
+  jn_part<EPT, TPR, R>(a, ab, a.slot_b, lane, sub, lds);
+  if (GATE == 1) jn_part<EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
   if (POST) {
-    jn_part<VEC, EPT, TPR, R>(a, apw, a.slot_pw, lane, sub, lds);
-    jn_part<VEC, EPT, TPR, R>(a, apb, a.slot_pb, lane, sub, lds);
+    jn_part<EPT, TPR, R>(a, apw, a.slot_pw, lane, sub, lds);
+    jn_part<EPT, TPR, R>(a, apb, a.slot_pb, lane, sub, lds);
   }
 }
 
@@ -396,14 +425,15 @@ __global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
 // ---------------------------------------------------------------------------
 
 // Lanes and elements a lane for a row of D.  Eight elements a lane keep the
-// backward kernel with Post at two waves a SIMD (16 took 256 registers and left
-// one); without Post 16 fit.  768 = 64 lanes of 12 without idle lanes.
+// backward kernel with Post, or in fp32, at two waves a SIMD (16 took 256
+// registers and left one); else 16 fit.  A lane's vectors are 16 bytes wide even where
+// that leaves lanes idle: rows of 768 as 64 lanes of 12 elements in vectors of
+// 8 bytes took 155 us backward where 64 lanes of 16 take 92 (49152 rows).
 struct JnShape {
   int ept, tpr;
 };
 static constexpr JnShape jn_shape(int64_t D, bool lean) {
   if (D <= 512) return {8, 64};
-  if (D <= 768) return {12, 64};
   if (D <= 1024) return lean ? JnShape{8, 128} : JnShape{16, 64};
   if (D <= 2048) return {8, 256};
   if (D <= 4096) return lean ? JnShape{8, 512} : JnShape{16, 256};
@@ -411,47 +441,40 @@ static constexpr JnShape jn_shape(int64_t D, bool lean) {
 }
 
 // DMAX: the longest row of the shape
-template <typename T, int VEC, bool BWD, bool POST, int GATE, int DMAX>
+template <typename T, bool BWD, bool POST, int GATE, int DMAX>
 static void jn_go(hipStream_t s, int grid, const JoinArgs& a) {
-  constexpr JnShape h = jn_shape(DMAX, BWD && POST);
-  constexpr int V = h.ept % VEC == 0 ? VEC : 4, N = JnBlock<h.tpr>::N;
+  constexpr JnShape h = jn_shape(DMAX, BWD && (POST || sizeof(T) == 4));
+  constexpr int N = JnBlock<h.tpr>::N;
   if constexpr (BWD)
-    hipLaunchKernelGGL((k_join_bwd<T, V, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
+    hipLaunchKernelGGL((k_join_bwd<T, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
   else
-    hipLaunchKernelGGL((k_join_fwd<T, V, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
+    hipLaunchKernelGGL((k_join_fwd<T, h.ept, h.tpr, POST, GATE>), dim3(grid), dim3(N), 0, s, a);
 }
 
-template <typename T, int VEC, bool BWD, bool POST, int GATE>
+template <typename T, bool BWD, bool POST, int GATE>
 static void jn_launch(hipStream_t s, int grid, const JoinArgs& a) {
-  if (a.D <= 512) jn_go<T, VEC, BWD, POST, GATE, 512>(s, grid, a);
-  else if (a.D <= 768) jn_go<T, VEC, BWD, POST, GATE, 768>(s, grid, a);
-  else if (a.D <= 1024) jn_go<T, VEC, BWD, POST, GATE, 1024>(s, grid, a);
-  else if (a.D <= 2048) jn_go<T, VEC, BWD, POST, GATE, 2048>(s, grid, a);
-  else if (a.D <= 4096) jn_go<T, VEC, BWD, POST, GATE, 4096>(s, grid, a);
-  else jn_go<T, VEC, BWD, POST, GATE, JN_MAXD>(s, grid, a);
-}
-
-template <typename T, int VEC, bool BWD>
-static void jn_form(hipStream_t s, int grid, const JoinArgs& a) {
-  const bool post = a.pw != nullptr;
-  if (post && a.gate_kind == 2) jn_launch<T, VEC, BWD, true, 2>(s, grid, a);
-  else if (post && a.gate_kind == 1) jn_launch<T, VEC, BWD, true, 1>(s, grid, a);
-  else if (post) jn_launch<T, VEC, BWD, true, 0>(s, grid, a);
-  else if (a.gate_kind == 2) jn_launch<T, VEC, BWD, false, 2>(s, grid, a);
-  else if (a.gate_kind == 1) jn_launch<T, VEC, BWD, false, 1>(s, grid, a);
-  else jn_launch<T, VEC, BWD, false, 0>(s, grid, a);
+  if (a.D <= 512) jn_go<T, BWD, POST, GATE, 512>(s, grid, a);
+  else if (a.D <= 1024) jn_go<T, BWD, POST, GATE, 1024>(s, grid, a);
+  else if (a.D <= 2048) jn_go<T, BWD, POST, GATE, 2048>(s, grid, a);
+  else if (a.D <= 4096) jn_go<T, BWD, POST, GATE, 4096>(s, grid, a);
+  else jn_go<T, BWD, POST, GATE, JN_MAXD>(s, grid, a);
 }
 
 template <typename T, bool BWD>
-static void jn_pick(hipStream_t s, int grid, const JoinArgs& a, bool vec) {
-  if (vec) jn_form<T, 16 / sizeof(T), BWD>(s, grid, a);
-  else jn_form<T, 1, BWD>(s, grid, a);
+static void jn_pick(hipStream_t s, int grid, const JoinArgs& a) {
+  const bool post = a.pw != nullptr;
+  if (post && a.gate_kind == 2) jn_launch<T, BWD, true, 2>(s, grid, a);
+  else if (post && a.gate_kind == 1) jn_launch<T, BWD, true, 1>(s, grid, a);
+  else if (post) jn_launch<T, BWD, true, 0>(s, grid, a);
+  else if (a.gate_kind == 2) jn_launch<T, BWD, false, 2>(s, grid, a);
+  else if (a.gate_kind == 1) jn_launch<T, BWD, false, 1>(s, grid, a);
+  else jn_launch<T, BWD, false, 0>(s, grid, a);
 }
 
 // Blocks of a group: the backward kernel's registers let 2048 waves be on the
 // chip at once; more would only write more parts.
-static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool post, bool backward) {
-  const JnShape h = jn_shape(D, post && backward);
+static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool lean, bool backward) {
+  const JnShape h = jn_shape(D, lean && backward);
   const int64_t rpb = h.tpr < 128 ? 256 / h.tpr : 1;
   const int64_t waves = h.tpr < 128 ? 4 : h.tpr / 64;
   const int64_t most = (backward ? 2048 : 8192) / waves / groups;
@@ -460,20 +483,15 @@ static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool post, boo
   return nb < 1 ? 1 : nb;
 }
 
-extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post) {
-  return jn_blocks(groups, rows, D, post != 0, true);
+extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post,
+                                  int bf16) {
+  return jn_blocks(groups, rows, D, post || !bf16, true);
 }
 
 static int jn_check(const JoinArgs& a, int64_t groups) {
   if (a.D < 1 || a.D > JN_MAXD || groups > 65530 || groups * a.nb > 0x7fffffff)
     return 9003;
   return 0;
-}
-
-static bool jn_vec(const void* const* p, int n, int D, int bf16) {
-  bool ok = D % (bf16 ? 8 : 4) == 0;
-  for (int i = 0; i < n; ++i) ok = ok && ((uintptr_t)p[i] & 15) == 0;
-  return ok;
 }
 
 // t: x, u, w, b, pw, pb, gate, y, h;  stats: my, ry, mu, ru
@@ -488,12 +506,11 @@ extern "C" int ps_join_fwd(void* stream, void* const* t, float* const* stats,
   a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
   a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
   a.gate_step = gate_step; a.scale = scale; a.eps = eps; a.invD = 1.0f / (float)D;
-  a.nb = (int)jn_blocks(groups, rows, D, a.pw != nullptr, false);
+  a.nb = (int)jn_blocks(groups, rows, D, false, false);
   if (int e = jn_check(a, groups)) return e;
-  const bool vec = jn_vec((const void* const*)t, 9, (int)D, bf16);
   const int grid = (int)(groups * a.nb);
-  if (bf16) jn_pick<__hip_bfloat16, false>((hipStream_t)stream, grid, a, vec);
-  else jn_pick<float, false>((hipStream_t)stream, grid, a, vec);
+  if (bf16) jn_pick<__hip_bfloat16, false>((hipStream_t)stream, grid, a);
+  else jn_pick<float, false>((hipStream_t)stream, grid, a);
   return (int)hipGetLastError();
 }
 
@@ -511,7 +528,7 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
   a.part = part;
   a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
   a.gate_step = gate_step; a.scale = scale; a.invD = 1.0f / (float)D;
-  a.nb = (int)jn_blocks(groups, rows, D, a.pw != nullptr, true);
+  a.nb = (int)ps_join_blocks(groups, rows, D, a.pw != nullptr, bf16);
   if (int e = jn_check(a, groups)) return e;
   JoinSums q{};
   int* slot[5] = {&a.slot_w, &a.slot_b, &a.slot_g, &a.slot_pw, &a.slot_pb};
@@ -519,11 +536,10 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
     *slot[i] = sums[i] ? a.slots : -1;
     if (sums[i]) q.out[a.slots++] = sums[i];
   }
-  const bool vec = jn_vec((const void* const*)t, 11, (int)D, bf16);
   const int grid = (int)(groups * a.nb);
   hipStream_t s = (hipStream_t)stream;
-  if (bf16) jn_pick<__hip_bfloat16, true>(s, grid, a, vec);
-  else jn_pick<float, true>(s, grid, a, vec);
+  if (bf16) jn_pick<__hip_bfloat16, true>(s, grid, a);
+  else jn_pick<float, true>(s, grid, a);
   if (int e = (int)hipGetLastError()) return e;
   if (a.slots == 0) return 0;
   q.part = part; q.slots = a.slots; q.slot_g = a.slot_g;

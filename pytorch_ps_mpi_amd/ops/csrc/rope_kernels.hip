@@ -46,8 +46,35 @@ template <typename T> __device__ __forceinline__ T rp_t(float v) { return (T)v; 
 template <> __device__ __forceinline__ __hip_bfloat16 rp_t(float v) { return __float2bfloat16(v); }
 template <> __device__ __forceinline__ __half rp_t(float v) { return __float2half(v); }
 
-// 16 bytes of T
-template <typename T> struct alignas(16) RpVec { T v[16 / sizeof(T)]; };
+// 16 bytes at any address that is a multiple of two: odd numbers of pairs,
+// strides and offsets are read as wide as others.
+typedef uint32_t rp_u4 __attribute__((ext_vector_type(4)));
+typedef rp_u4 rp_u4_any __attribute__((aligned(2)));
+template <typename T> struct RpVec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+  // `n` elements, all of them in one access
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= N) {
+      const rp_u4 u = *(const rp_u4_any*)p;
+      __builtin_memcpy(v, &u, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = j < n ? p[j] : rp_t<T>(0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n) const {
+    if (n >= N) {
+      rp_u4 u;
+      __builtin_memcpy(&u, v, 16);
+      *(rp_u4_any*)p = u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) p[j] = v[j];
+    }
+  }
+};
 
 __device__ __forceinline__ void rp_angles(const RopeArgs& a, int64_t row0,
                                           int toks, float2* cs) {
@@ -66,20 +93,20 @@ __device__ __forceinline__ void rp_angles(const RopeArgs& a, int64_t row0,
   }
 }
 
-// VEC elements of 16 bytes at once; VEC == 1: any size and alignment.
-// Half-split: item c holds pairs [c*VEC, c*VEC+VEC), that is two vectors.
-// Interleaved: item c holds elements [c*VEC, ...), VEC/2 pairs.
-template <typename T, int VEC, bool INTER>
+// An item is a vector of V elements.  Half-split: item c holds pairs cV and on,
+// that is two vectors P apart.  Interleaved: elements cV and on, V/2 pairs.
+// Behind them the items that pass through.
+template <typename T, bool INTER>
 __global__ void __launch_bounds__(RP_BLOCK) k_rope(const RopeArgs a) {
   extern __shared__ float2 cs[];
+  constexpr int V = RpVec<T>::N;
   const int64_t row0 = (int64_t)blockIdx.x * RP_TOK;
   const int toks = (int)min((int64_t)RP_TOK, a.rows - row0);
   rp_angles(a, row0, toks, cs);
   __syncthreads();
   const int P = a.P, D = a.D;
-  const int turn = INTER ? (VEC == 1 ? P : 2 * P / VEC) : P / VEC;
-  const int rest = (D - 2 * P) / VEC;  // items that pass through
-  const int per = turn + rest;
+  const int turn = ((INTER ? 2 * P : P) + V - 1) / V;
+  const int per = turn + (D - 2 * P + V - 1) / V;
   const int heads = a.t[0].H + a.t[1].H;
   const int total = toks * heads * per;
   for (int i = threadIdx.x; i < total; i += RP_BLOCK) {
@@ -94,57 +121,47 @@ __global__ void __launch_bounds__(RP_BLOCK) k_rope(const RopeArgs a) {
     const T* x = (const T*)w.x + b * w.sB + n * w.sN + h * w.sH;
     T* y = (T*)w.y + (row * w.H + h) * D;
     const float2* tc = cs + t * P;
+    RpVec<T> u, v;
     if (c >= turn) {
-      const int e = 2 * P + (c - turn) * VEC;
-      if (VEC == 1) y[e] = x[e];
-      else *(RpVec<T>*)(y + e) = *(const RpVec<T>*)(x + e);
-    } else if (VEC == 1) {
-      const int ia = INTER ? 2 * c : c, ib = INTER ? 2 * c + 1 : P + c;
-      const float va = rp_f(x[ia]), vb = rp_f(x[ib]);
-      const float2 k = tc[c];
-      y[ia] = rp_t<T>(va * k.x - vb * k.y);
-      y[ib] = rp_t<T>(va * k.y + vb * k.x);
+      const int e = 2 * P + (c - turn) * V;
+      u.load(x + e, D - e);
+      u.store(y + e, D - e);
     } else if (INTER) {
-      const RpVec<T> v = *(const RpVec<T>*)(x + c * VEC);
-      RpVec<T> o;
+      const int e = c * V;
+      u.load(x + e, 2 * P - e);
 #pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
-        const float2 k = tc[c * (VEC / 2) + j / 2];
-        const float va = rp_f(v.v[j]), vb = rp_f(v.v[j + 1]);
-        o.v[j] = rp_t<T>(va * k.x - vb * k.y);
-        o.v[j + 1] = rp_t<T>(va * k.y + vb * k.x);
+      for (int j = 0; j < V; j += 2) {
+        const float2 k = tc[min(e / 2 + j / 2, P - 1)];
+        const float va = rp_f(u.v[j]), vb = rp_f(u.v[j + 1]);
+        u.v[j] = rp_t<T>(va * k.x - vb * k.y);
+        u.v[j + 1] = rp_t<T>(va * k.y + vb * k.x);
       }
-      *(RpVec<T>*)(y + c * VEC) = o;
+      u.store(y + e, 2 * P - e);
     } else {
-      const RpVec<T> u = *(const RpVec<T>*)(x + c * VEC);
-      const RpVec<T> v = *(const RpVec<T>*)(x + P + c * VEC);
-      RpVec<T> o, q;
+      const int e = c * V;
+      u.load(x + e, P - e);
+      v.load(x + P + e, P - e);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float2 k = tc[c * VEC + j];
+      for (int j = 0; j < V; ++j) {
+        const float2 k = tc[min(e + j, P - 1)];
         const float va = rp_f(u.v[j]), vb = rp_f(v.v[j]);
-        o.v[j] = rp_t<T>(va * k.x - vb * k.y);
-        q.v[j] = rp_t<T>(va * k.y + vb * k.x);
+        u.v[j] = rp_t<T>(va * k.x - vb * k.y);
+        v.v[j] = rp_t<T>(va * k.y + vb * k.x);
       }
-      *(RpVec<T>*)(y + c * VEC) = o;
-      *(RpVec<T>*)(y + P + c * VEC) = q;
+      u.store(y + e, P - e);
+      v.store(y + P + e, P - e);
     }
   }
 }
 
 template <typename T>
-static void rp_launch(hipStream_t s, const RopeArgs& a, bool vec, bool inter) {
-  constexpr int V = 16 / sizeof(T);
+static void rp_launch(hipStream_t s, const RopeArgs& a, bool inter) {
   const int grid = (int)((a.rows + RP_TOK - 1) / RP_TOK);
   const size_t lds = (size_t)RP_TOK * a.P * sizeof(float2);
-  if (vec && inter)
-    hipLaunchKernelGGL((k_rope<T, V, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
-  else if (vec)
-    hipLaunchKernelGGL((k_rope<T, V, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
-  else if (inter)
-    hipLaunchKernelGGL((k_rope<T, 1, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+  if (inter)
+    hipLaunchKernelGGL((k_rope<T, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
   else
-    hipLaunchKernelGGL((k_rope<T, 1, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+    hipLaunchKernelGGL((k_rope<T, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
 }
 
 // strides: q's B, N, H, k's B, N, H, pos's axis, B, N.  dtype: 0 bf16, 1 fp16,
@@ -171,14 +188,9 @@ extern "C" int ps_rope(void* stream, const void* q, const void* k, void* yq,
   for (int i = 0; i < 3; ++i) a.start[i] = start[i];
   a.sign = backward ? -1.0f : 1.0f;
   for (int i = 0; i < P; ++i) a.rev[i] = rev[i];
-  const int V = dtype == 2 ? 4 : 8;
-  bool vec = D % V == 0 && (inter ? 2 * P : P) % V == 0;
-  for (int i = 0; i < 6; ++i) vec = vec && strides[i] % V == 0;
-  for (const void* p : {q, k, (const void*)yq, (const void*)yk})
-    vec = vec && ((uintptr_t)p & 15) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == 0) rp_launch<__hip_bfloat16>(s, a, vec, inter);
-  else if (dtype == 1) rp_launch<__half>(s, a, vec, inter);
-  else rp_launch<float>(s, a, vec, inter);
+  if (dtype == 0) rp_launch<__hip_bfloat16>(s, a, inter);
+  else if (dtype == 1) rp_launch<__half>(s, a, inter);
+  else rp_launch<float>(s, a, inter);
   return (int)hipGetLastError();
 }
