@@ -435,13 +435,13 @@ void join_fwd(OptTensors t, at::Tensor stats, int64_t groups, int64_t rows,
            "join_fwd");
 }
 
-// t: u, w, pw, pb, gate, y, dy, dh, dx, du, dgate; sums: dw, db, dgate, dpw,
+// t: u, w, pw, pb, gate, x, dy, dh, dx, du, dgate; sums: dw, db, dgate, dpw,
 // dpb
 void join_bwd(OptTensors t, at::Tensor stats, OptTensors sums, at::Tensor part,
               int64_t groups, int64_t rows, int64_t D, bool layer,
               int64_t gate_kind, int64_t gate_step, double scale) {
   TORCH_CHECK(t.size() == 11 && t[0] && t[1] && t[5] && t[8] && t[9],
-              "join_bwd: u, w, y, dx, du wanted");
+              "join_bwd: u, w, x, dx, du wanted");
   TORCH_CHECK(gate_kind == 0 || t[4], "join_bwd: gate wanted");
   const at::Tensor& u = *t[0];
   TORCH_CHECK(is_bf16(u) || u.scalar_type() == at::kFloat, "bf16 or fp32");
@@ -496,7 +496,7 @@ struct GatedResidual : torch::autograd::Function<GatedResidual> {
                            x.options().dtype(at::kFloat));
     join_fwd({x, u, w, opt(b), opt(pw), opt(pb), opt(gate), y, h}, stats,
              groups, rows, D, layer, gate_kind, step, scale, eps);
-    ctx->save_for_backward({y, u, w, gate, pw, pb, stats});
+    ctx->save_for_backward({x, u, w, gate, pw, pb, stats});
     ctx->saved_data["cfg"] =
         std::vector<int64_t>{groups, rows, D, layer, gate_kind, step,
                              b.defined()};
@@ -511,11 +511,11 @@ struct GatedResidual : torch::autograd::Function<GatedResidual> {
     torch::autograd::variable_list out(12);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    const auto &y = s[0], &u = s[1], &w = s[2], &gate = s[3], &pw = s[4],
+    const auto &x = s[0], &u = s[1], &w = s[2], &gate = s[3], &pw = s[4],
                &pb = s[5], &stats = s[6];
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     const int64_t groups = cfg[0], rows = cfg[1], D = cfg[2], kind = cfg[4];
-    const c10::DeviceGuard guard(y.device());
+    const c10::DeviceGuard guard(x.device());
     const Opt dy = g[0].defined() ? Opt(g[0].contiguous()) : Opt();
     const Opt dh = g[1].defined() ? Opt(g[1].contiguous()) : Opt();
     // inputs that are there, in order: x, u, w, b, gate, pw, pb
@@ -525,7 +525,7 @@ struct GatedResidual : torch::autograd::Function<GatedResidual> {
     size_t edge = 0;
     for (int i = 0; i < 7; ++i)
       need[i] = there[i] && ctx->needs_input_grad(edge++);
-    out[0] = at::empty_like(y);
+    out[0] = at::empty_like(x);
     out[1] = at::empty_like(u);
     // without dh the last norm's parameters get no gradient
     if (need[2] && dh) out[2] = at::empty_like(w);
@@ -540,8 +540,8 @@ struct GatedResidual : torch::autograd::Function<GatedResidual> {
                            ps_join_blocks(groups, rows, D, pw.defined(),
                                           is_bf16(u)) *
                            slots * D},
-                          y.options().dtype(at::kFloat));
-    join_bwd({u, w, opt(pw), opt(pb), opt(gate), y, dy, dh, out[0], out[1],
+                          x.options().dtype(at::kFloat));
+    join_bwd({u, w, opt(pw), opt(pb), opt(gate), x, dy, dh, out[0], out[1],
               kind == 2 ? opt(out[4]) : Opt()},
              stats, {opt(out[2]), opt(out[3]), vec, opt(out[5]), opt(out[6])},
              part, groups, rows, D, cfg[3] != 0, kind, cfg[5],

@@ -7,11 +7,11 @@
 // one vector for all rows, one for each sample, or a whole tensor.
 //
 // Bound by HBM: the forward pass reads x, u and writes y, h; the backward pass
-// reads y, u, dy, dh and writes dx, du, everything else of a row stays in
+// reads x, u, dy, dh and writes dx, du, everything else of a row stays in
 // registers.  A row belongs to one wave (D <= 1024) or one block (D <= 8192),
 // at most 16 elements a lane.  Means and variances in fp32, the variance about
-// the mean (two sums), h from the unrounded y; the backward pass takes the
-// rounded y, whose error of half a step is averaged like that of any input.
+// the mean (two sums).  Both passes take y before its rounding: the backward
+// one computes it again from x and u, which cost what reading y would.
 //
 // Sums over rows (weights, biases, gate): each block keeps its rows' sums in
 // registers, writes them once, and a second kernel adds the blocks' parts in
@@ -287,12 +287,12 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
   w.load(a.w, 0, lane, D);
   if (POST) {
     pw.load(a.pw, 0, lane, D);
-    if (GATE) pb.load(a.pb, 0, lane, D);
+    pb.load(a.pb, 0, lane, D);
   }
   if (GATE == 1) gate.load(a.gate, group * a.gate_step, lane, D);
   const int64_t step = (int64_t)a.nb * RPB;
   int64_t i = (int64_t)blk * RPB + sub;
-  R yn, un, dyn, dhn, gn;  // the next row's, on their way
+  R xn, un, dyn, dhn, gn;  // the next row's, on their way
   float m1n = 0.0f, r1n = 0.0f, m2n = 0.0f, r2n = 1.0f;
   auto load = [&](int64_t at) {
     const int64_t row = group * a.rows + at, off = row * D;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
       m2n = a.mu[row];
       r2n = a.ru[row];
     }
-    yn.load(a.y, off, lane, D);
+    xn.load(a.x, off, lane, D);
     dhn.load(a.dh, off, lane, D);
     dyn.load(a.dy, off, lane, D);
     un.load(a.u, off, lane, D);
@@ -314,15 +314,20 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
   for (; i < a.rows; i += step) {
     const int64_t row = group * a.rows + i, off = row * D;
     if (!AHEAD) load(i);
-    R y = yn, u = un, dy = dyn, dh = dhn;
+    R x = xn, u = un, dy = dyn, dh = dhn;
     if (GATE == 2) gate = gn;
     const float m1 = m1n, r1 = r1n, m2 = m2n, r2 = r2n;
     if (AHEAD && i + step < a.rows) load(i + step);
     float t[EPT];  // the whole gradient of y
+    float y[EPT];  // y's normed value
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
-      const float xh = (y.get(j) - m1) * r1, g = dh.get(j);
+      float n = u.get(j);
+      if (POST) n = fmaf((n - m2) * r2, pw.get(j), pb.get(j));
+      if (GATE) n *= gate.get(j);
+      const float xh = (fmaf(a.scale, x.get(j), n) - m1) * r1, g = dh.get(j);
+      y[j] = xh;
       aw[j] = fmaf(g, xh, aw[j]);
       ab[j] += g;
       t[j] = g * w.get(j);
@@ -330,13 +335,13 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
       s2 = fmaf(t[j], xh, s2);
     }
     float2 s = jn_sum2<TPR>(s1, s2, red, turn);
-    float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD * r1;
+    float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
-      t[j] = fmaf(r1, fmaf(m1 - y.get(j), c2, t[j] - c1), dy.get(j));
-      y.set(j, a.scale * t[j]);
+      t[j] = fmaf(r1, fmaf(-y[j], c2, t[j] - c1), dy.get(j));
+      x.set(j, a.scale * t[j]);
     }
-    y.store(a.dx, off, lane, D);
+    x.store(a.dx, off, lane, D);
     s1 = s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
@@ -515,7 +520,7 @@ extern "C" int ps_join_fwd(void* stream, void* const* t, float* const* stats,
   return (int)hipGetLastError();
 }
 
-// t: u, w, pw, pb, gate, y, dy, dh, dx, du, dgate (whole tensor);
+// t: u, w, pw, pb, gate, x, dy, dh, dx, du, dgate (whole tensor);
 // sums: dw, db, dgate (vectors), dpw, dpb — null where not wanted.
 extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
                            void* const* sums, float* part, int bf16,
@@ -523,7 +528,7 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
                            int gate_kind, int64_t gate_step, float scale) {
   if (groups <= 0 || rows <= 0) return 0;
   JoinArgs a{};
-  a.u = t[0]; a.w = t[1]; a.pw = t[2]; a.pb = t[3]; a.gate = t[4]; a.y = t[5];
+  a.u = t[0]; a.w = t[1]; a.pw = t[2]; a.pb = t[3]; a.gate = t[4]; a.x = t[5];
   a.dy = t[6]; a.dh = t[7]; a.dx = t[8]; a.du = t[9]; a.dgate = t[10];
   a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
   a.part = part;

@@ -1,9 +1,8 @@
 """fused_gated_residual kernels against 64 bits (@gpu).
 
 Bounds.  e is half a step of the type, S = 64 * 2^-24 covers fp32 arithmetic
-(sums over lanes, waves and blocks: some 30 roundings).  The backward pass has
-y rounded: its normed value is off by at most e |y| r, which moves the two
-projections; `_bounds` carries that through term by term.
+(sums over lanes, waves and blocks: some 30 roundings); `_bounds` carries the
+error of the normed values through the backward pass term by term.
 """
 
 import pytest
@@ -54,7 +53,7 @@ def _bounds(d, want, dtype, scale, kind, eps):
     tol = {"y": e * y.abs() + S * (mag + gate.abs()),
            "h": e * want["h"].abs() + S * (
                (mag + top) * r * d["w"].abs() + want["h"].abs() + 1)}
-    off = e * y.abs() * r + S * (1 + hat.abs())   # of the normed value
+    off = S * ((mag + top) * r + hat.abs())       # of the normed value
     k = (d["gh"] * d["w"])
     c2 = mean(k * hat).abs()
     et = r * (off * c2 + hat.abs() * mean(k.abs() * off)
