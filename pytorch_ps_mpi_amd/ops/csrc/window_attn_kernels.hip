@@ -434,6 +434,18 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
     scores(ldk, 0, s0);
     wa_feed<D / 16, D / 16, 4, 1>();
   }
+  // Nothing is read where the next tile arrives (`to`): the compiler need not
+  // wait for it.
+  auto first = [&](const char* __restrict__ tv, const char* __restrict__ tk,
+                   char* __restrict__ to, bool more, int n0, int k0, int seen1) {
+    if (more) mv.go(n0, w.len, to, wave);
+    strip(s0, seen0, k0, tv, 0, s1, seen1, tk, 1);
+  };
+  auto second = [&](const char* __restrict__ tv, const char* __restrict__ tk,
+                    char* __restrict__ to, bool more, int n0, int k0, int seen1, int seen2) {
+    if (more) mk.go(n0, w.len, to, wave);
+    strip(s1, seen1, k0, tv, 1, s0, seen2, tk, 0);
+  };
   // o: 0 or TILE, where this tile stands
   auto step = [&](int it, int o) {
     const int k0 = w.tile(it) * WA_T;
@@ -442,11 +454,10 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
     const int seen1 = wa_seen(a, w.wrow, k0 + 32, 32);
     const int seen2 = more ? wa_seen(a, w.wrow, n0, 32) : 0;
     if (it) wa_sync();
-    if (more) mv.go(n0, w.len, ldv + (TILE - o), wave);
-    strip(s0, seen0, k0, ldv + o, 0, s1, seen1, ldk + o, 1);
+    first(ldv + o, ldk + o, ldv + (TILE - o), more, n0, k0, seen1);
     wa_sync();  // this tile's keys have been read
-    if (more2) mk.go(w.tile(it + 2) * WA_T, w.len, ldk + o, wave);
-    strip(s1, seen1, k0 + 32, ldv + o, 1, s0, seen2, ldk + (TILE - o), 0);
+    second(ldv + o, ldk + (TILE - o), ldk + o, more2, more2 ? w.tile(it + 2) * WA_T : 0,
+           k0 + 32, seen1, seen2);
     seen0 = seen2;
   };
   for (int it = 0; it < w.count; it += 2) {
@@ -512,7 +523,8 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
   mk.go(w.tile(0) * WA_T, w.len, lds, wave);
   mv.go(w.tile(0) * WA_T, w.len, lds + TILE, wave);
   const float c = a.scale * WA_LOG2E;
-  auto step = [&](int it, char* mine, char* next) {
+  // nothing is read where the next tile arrives: the compiler need not wait
+  auto step = [&](int it, char* __restrict__ mine, char* __restrict__ next) {
     char* tk = mine;
     char* tv = mine + TILE;
     const int k0 = w.tile(it) * WA_T;
@@ -673,7 +685,8 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
     load(lds);
     keep(lds);
     int at_tile = 0;
-    auto step = [&](int it, char* buf, char* next) {
+    // nothing is read where the next tile arrives: the compiler need not wait
+    auto step = [&](int it, char* __restrict__ buf, char* __restrict__ next) {
       char* tq = buf;
       char* tg = buf + TILE;
       float* stat = (float*)(buf + 2 * TILE);
