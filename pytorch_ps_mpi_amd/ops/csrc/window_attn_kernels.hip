@@ -69,6 +69,8 @@ struct WaArgs {
   const int32_t* lengths;       // [B], or null
   int B, H, KV, N, window, sinks;
   int strips, slots;            // strips of 32 first tokens, waves that share one's rows
+  int split;                    // blocks that share the rows of 128 keys
+  float* splits;                // their sums, where there is more than one
   float scale;
 };
 
@@ -604,6 +606,11 @@ template <int D>
 __device__ __forceinline__ float* wa_part(const WaArgs& a, int u, int strip, int slot) {
   return a.part + (((int64_t)u * a.strips + strip) * (1 + a.slots) + slot) * 2 * 32 * D;
 }
+// fp32 sums [sequence and key head][128 keys][share][dK, dV][128][D]
+template <int D>
+__device__ __forceinline__ float* wa_split(const WaArgs& a, int u, int nkb, int kblk, int share) {
+  return a.splits + (((int64_t)u * nkb + kblk) * a.split + share) * 2 * WA_KB * D;
+}
 template <int DT>
 __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int half) {
 #pragma unroll
@@ -615,14 +622,10 @@ __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int h
     }
 }
 
-template <int D>
-struct WaDkv {
-  static constexpr int PARTS = D == 128 ? 2 : 1, NT = WA_BLOCK * PARTS;
-};
-
-template <int D>
-__global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
-  constexpr int PARTS = WaDkv<D>::PARTS, NT = WaDkv<D>::NT;
+template <int D, int PARTS>
+__global__ void __launch_bounds__(PARTS * WA_BLOCK, PARTS == 1 ? 3 : 2)
+k_wa_dkv(const WaArgs a) {
+  constexpr int NT = PARTS * WA_BLOCK;
   constexpr int TILE = WA_T * D * 2, BUF = 2 * TILE + 2 * WA_T * 4;
   constexpr int H2 = D / PARTS, DT = H2 / 32;  // this wave's part of D
   // two buffers of Q, dO and the rows' statistics; P and dS on their way
@@ -630,18 +633,21 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = wa_wave(), part = PARTS == 1 ? 0 : wave >> 2;
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
-  const int id = wa_block(), u = id / nkb, k0 = (id - u * nkb) * WA_KB;
+  const int id = wa_block() / a.split, share = wa_block() - id * a.split;
+  const int u = id / nkb, k0 = (id - u * nkb) * WA_KB;
   const int b = u / a.KV, kv = u - b * a.KV, G = a.H / a.KV;
   const int len = wa_len(a, b);
   // the rows, in tiles, of each head: the window's
   const int t0 = k0 / WA_T, total = max(wa_behind(a, k0, len) - t0, 0);
-  const int it1 = total * G;  // (head, tile) pairs
+  // (head, tile) pairs: this block's share of them
+  const int each = (total * G + a.split - 1) / a.split;
+  const int it0 = min(share * each, total * G), it1 = min(it0 + each, total * G);
   const int wk = k0 + (wave & 3) * 32;   // this wave's first key
   const int key = wk + col;
   wa_f16 ak[DT], av[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) ak[t] = av[t] = (wa_f16)(0.0f);
-  if (it1 > 0) {
+  if (it0 < it1) {
     wa_bf8 kf[D / 16], vf[D / 16];
     const int at = min(key, len - 1);
     wa_row<D>(a.k.p + b * a.k.sB + kv * a.k.sH + at * a.k.sN, half, kf);
@@ -656,13 +662,14 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
     float sl = 0.0f, sd = 0.0f;
     const float c = a.scale * WA_LOG2E;
     const bool sinkkey = key < a.sinks;
-    int head = kv * G, tile = 0;  // what travels next
+    int head = kv * G + it0 / total, tile = it0 % total;  // what travels next
+    auto of_head = [&]() {
+      mq.from(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN);
+      mg.from(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN);
+    };
     auto load = [&](char* to) {
       const int r0 = (t0 + tile) * WA_T;
-      if (tile == 0) {
-        mq.from(a.q.p + b * a.q.sB + head * a.q.sH, a.q.sN);
-        mg.from(a.go.p + b * a.go.sB + head * a.go.sH, a.go.sN);
-      }
+      if (tile == 0) of_head();
       mq.go(r0, len, to, wave);
       mg.go(r0, len, to + TILE, wave);
       if (threadIdx.x < WA_T) {
@@ -682,9 +689,10 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
         ((float*)(to + 2 * TILE))[WA_T + threadIdx.x] = sd;
       }
     };
+    int at_tile = tile;
+    of_head();
     load(lds);
     keep(lds);
-    int at_tile = 0;
     // nothing is read where the next tile arrives: the compiler need not wait
     auto step = [&](int it, char* __restrict__ buf, char* __restrict__ next) {
       char* tq = buf;
@@ -759,10 +767,16 @@ __global__ void __launch_bounds__(WaDkv<D>::NT, 2) k_wa_dkv(const WaArgs a) {
       }
       if (more) keep(next);
     };
-    for (int it = 0; it < it1; it += 2) {
+    for (int it = it0; it < it1; it += 2) {
       step(it, lds, lds + BUF);
       if (it + 1 < it1) step(it + 1, lds + BUF, lds);
     }
+  }
+  if (a.split > 1) {
+    float* p = wa_split<D>(a, u, nkb, k0 / WA_KB, share) + (key - k0) * D + part * H2;
+    wa_store_part<DT>(p, ak, half);
+    wa_store_part<DT>(p + WA_KB * D, av, half);
+    return;
   }
   const bool split = a.slots > 0 && key < a.sinks;
   if (split) {
@@ -865,20 +879,48 @@ __global__ void __launch_bounds__(WA_BLOCK, D == 64 ? 2 : 1) k_wa_sink(const WaA
   }
 }
 
-// dK and dV of the first tokens: the parts in fixed order, 1024 / D at a time.
+// dK and dV from parts, in fixed order.  The first blocks take a first token
+// each, 1024 / D parts at a time; the others, where blocks shared the rows of
+// 128 keys, 4096 / D of the remaining keys each.
 template <int D>
-__global__ void __launch_bounds__(1024) k_wa_sink_sum(const WaArgs a) {
+__global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a) {
   constexpr int W = 1024 / D;
   __shared__ float lds[2][W][D];
-  const int key = blockIdx.x, u = blockIdx.y;
-  const int b = u / a.KV, kv = u - b * a.KV;
-  const int d = threadIdx.x % D, w = threadIdx.x / D;
+  const int first = a.slots > 0 ? a.sinks : 0;  // keys with parts of strips
+  const int u = blockIdx.y, b = u / a.KV, kv = u - b * a.KV;
+  const int nkb = (a.N + WA_KB - 1) / WA_KB;
+  if ((int)blockIdx.x >= first) {
+    const int key = first + ((int)blockIdx.x - first) * (4096 / D) + threadIdx.x / (D / 4);
+    const int d = threadIdx.x % (D / 4) * 4;
+    if (key >= a.N) return;
+    const float* p = wa_split<D>(a, u, nkb, key / WA_KB, 0) + (key % WA_KB) * D + d;
+    float4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+    for (int s = 0; s < a.split; ++s, p += 2 * WA_KB * D) {
+      const float4 x = *(const float4*)p, y = *(const float4*)(p + WA_KB * D);
+      k.x += x.x; k.y += x.y; k.z += x.z; k.w += x.w;
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+    const int64_t off = (((int64_t)b * a.N + key) * a.KV + kv) * D + d;
+    const uint2 ok = {wa_pack(k.x * a.scale, k.y * a.scale), wa_pack(k.z * a.scale, k.w * a.scale)};
+    const uint2 ov = {wa_pack(v.x, v.y), wa_pack(v.z, v.w)};
+    *(uint2*)(a.dk + off) = ok;
+    *(uint2*)(a.dv + off) = ov;
+    return;
+  }
+  const int key = blockIdx.x, d = threadIdx.x % D, w = threadIdx.x / D;
   float sk = 0.0f, sv = 0.0f;
-  for (int s = w; s <= a.slots; s += W) {
+  // part 0 is the rows' by the window, unless those are shared out themselves
+  for (int s = w + (a.split > 1); s <= a.slots; s += W) {
     const float* p = wa_part<D>(a, u, key / 32, s) + (key % 32) * D + d;
     sk += p[0];
     sv += p[32 * D];
   }
+  if (a.split > 1)
+    for (int s = w; s < a.split; s += W) {
+      const float* p = wa_split<D>(a, u, nkb, key / WA_KB, s) + (key % WA_KB) * D + d;
+      sk += p[0];
+      sv += p[WA_KB * D];
+    }
   lds[0][w][d] = sk;
   lds[1][w][d] = sv;
   __syncthreads();
@@ -907,13 +949,31 @@ static int wa_slots(int64_t U, int64_t G, int64_t N, int64_t window, int64_t sin
   return (int)((n < 4 ? 4 : n) / 4 * 4);
 }
 
+// Blocks that share the rows of 128 keys where there are fewer of those than
+// CUs: one round of blocks, with at least four (head, tile) pairs each.  6 sequences of
+// 777, 8 over 2 heads of 128, window 100: 43 us in 84 blocks, _SPLIT_.
+static int wa_splits(int64_t U, int64_t G, int64_t N, int64_t window) {
+  const int64_t blocks = U * ((N + WA_KB - 1) / WA_KB);
+  const int64_t rows = window + WA_KB < N ? window + WA_KB : N;
+  const int64_t most = G * ((rows + WA_T - 1) / WA_T) / 4;
+  int64_t n = 256 / blocks;
+  if (n > most) n = most;
+  return (int)(n < 1 ? 1 : n);
+}
+
+static int64_t wa_slot_floats(int64_t U, int64_t D, int64_t sinks, int64_t slots) {
+  return slots ? U * ((sinks + 31) / 32) * (1 + slots) * 2 * 32 * D : 0;
+}
+
 extern "C" int64_t ps_wa_part_floats(int64_t B, int64_t H, int64_t KV, int64_t N,
                                      int64_t D, int64_t window, int64_t sinks) {
   if (B <= 0 || KV <= 0 || N <= 0) return 0;
+  const int64_t U = B * KV, G = H / KV;
   if (sinks > N) sinks = N;
-  const int64_t slots = wa_slots(B * KV, H / KV, N, window, sinks);
-  if (slots == 0) return 0;
-  return B * KV * ((sinks + 31) / 32) * (1 + slots) * 2 * 32 * D;
+  if (window > N) window = N;
+  const int64_t split = wa_splits(U, G, N, window);
+  return wa_slot_floats(U, D, sinks, wa_slots(U, G, N, window, sinks)) +
+         (split > 1 ? U * ((N + WA_KB - 1) / WA_KB) * split * 2 * WA_KB * D : 0);
 }
 
 static int wa_fill(WaArgs& a, const int64_t* st, int64_t B, int64_t H, int64_t KV,
@@ -931,6 +991,7 @@ static int wa_fill(WaArgs& a, const int64_t* st, int64_t B, int64_t H, int64_t K
   a.sinks = (int)(sinks < N ? sinks : N);
   a.strips = (a.sinks + 31) / 32;
   a.slots = wa_slots(B * KV, H / KV, N, a.window, a.sinks);
+  a.split = wa_splits(B * KV, H / KV, N, a.window);
   a.scale = scale;
   a.lengths = lengths;
   return 0;
@@ -978,27 +1039,34 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
   a.dq = (__bf16*)dq; a.dk = (__bf16*)dk; a.dv = (__bf16*)dv;
   const int gw = wa_heads_a_block(H / KV);
   const int64_t grid = wa_row_grid(B, H, N, gw);
-  const int64_t kgrid = B * KV * ((N + WA_KB - 1) / WA_KB);
+  a.splits = part + wa_slot_floats(B * KV, D, a.sinks, a.slots);
+  const int64_t kgrid = B * KV * ((N + WA_KB - 1) / WA_KB) * a.split;
   const int64_t sgrid = B * KV * a.strips * (a.slots / 4);
+  // blocks that add parts: see k_wa_sum
+  const int64_t first = a.slots ? a.sinks : 0;
+  const int64_t sums = first + (a.split > 1 ? (N - first + 4096 / D - 1) / (4096 / D) : 0);
   if (grid > 0x7fffffff || kgrid > 0x7fffffff || sgrid > 0x7fffffff ||
       B * KV > 65535 || (D != 64 && D != 128))
     return 9003;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 sums((unsigned)a.sinks, (unsigned)(B * KV));
+  const dim3 rows((unsigned)grid), keys((unsigned)kgrid), strips((unsigned)sgrid);
+  const dim3 adds((unsigned)sums, (unsigned)(B * KV));
   if (D == 64) {
-    hipLaunchKernelGGL((k_wa_dq<64>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
-    hipLaunchKernelGGL((k_wa_dkv<64>), dim3((unsigned)kgrid), dim3(WaDkv<64>::NT), 0, s, a);
-    if (a.slots) {
-      hipLaunchKernelGGL((k_wa_sink<64>), dim3((unsigned)sgrid), dim3(WA_BLOCK), 0, s, a);
-      hipLaunchKernelGGL((k_wa_sink_sum<64>), sums, dim3(1024), 0, s, a);
-    }
+    hipLaunchKernelGGL((k_wa_dq<64>), rows, dim3(WA_BLOCK), 0, s, a, gw);
+    // Pairs of waves where blocks do not fill the chip by themselves (16 key
+    // heads of 2048: 66 us against 102), else one wave for both (96 of 1024:
+    // 31 us against 41).
+    if (kgrid < 512)
+      hipLaunchKernelGGL((k_wa_dkv<64, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
+    else
+      hipLaunchKernelGGL((k_wa_dkv<64, 1>), keys, dim3(WA_BLOCK), 0, s, a);
+    if (a.slots) hipLaunchKernelGGL((k_wa_sink<64>), strips, dim3(WA_BLOCK), 0, s, a);
+    if (sums) hipLaunchKernelGGL((k_wa_sum<64>), adds, dim3(1024), 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_wa_dq<128>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
-    hipLaunchKernelGGL((k_wa_dkv<128>), dim3((unsigned)kgrid), dim3(WaDkv<128>::NT), 0, s, a);
-    if (a.slots) {
-      hipLaunchKernelGGL((k_wa_sink<128>), dim3((unsigned)sgrid), dim3(WA_BLOCK), 0, s, a);
-      hipLaunchKernelGGL((k_wa_sink_sum<128>), sums, dim3(1024), 0, s, a);
-    }
+    hipLaunchKernelGGL((k_wa_dq<128>), rows, dim3(WA_BLOCK), 0, s, a, gw);
+    hipLaunchKernelGGL((k_wa_dkv<128, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
+    if (a.slots) hipLaunchKernelGGL((k_wa_sink<128>), strips, dim3(WA_BLOCK), 0, s, a);
+    if (sums) hipLaunchKernelGGL((k_wa_sum<128>), adds, dim3(1024), 0, s, a);
   }
   return (int)hipGetLastError();
 }
