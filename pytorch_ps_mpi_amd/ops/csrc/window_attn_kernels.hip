@@ -32,9 +32,8 @@
 // the group, so that shared heads are summed in registers, without atomics.
 //
 // The first tokens are seen by all rows: their dK/dV would be one block's work
-// of N rows among blocks of `window` rows.  The rows behind the window go to a
-// kernel of their own, whose waves take a strip of 32 first tokens and some of
-// the rows each; a last kernel adds their parts in fixed order.
+// of N rows among blocks of `window` rows.  The rows behind the window are
+// shared out over further blocks; a last kernel adds their parts in fixed order.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -68,7 +67,8 @@ struct WaArgs {
   float* part;                  // dK, dV parts of the first tokens
   const int32_t* lengths;       // [B], or null
   int B, H, KV, N, window, sinks;
-  int strips, slots;            // strips of 32 first tokens, waves that share one's rows
+  int strips, slots;            // strips of 32 first tokens; blocks that share the rows
+                                // behind the window of 128 of them
   int split;                    // blocks that share the rows of 128 keys
   float* splits;                // their sums, where there is more than one
   float scale;
@@ -272,8 +272,8 @@ __device__ __forceinline__ int wa_len(const WaArgs& a, int b) {
 
 // Blocks go to the 8 XCDs in turn, each with an L2 of its own: give every XCD a
 // stretch of neighbouring blocks, which read the same tiles.
-__device__ __forceinline__ int wa_block() {
-  const int n = gridDim.x, x = blockIdx.x & 7;
+__device__ __forceinline__ int wa_block(int n) {
+  const int x = blockIdx.x & 7;
   return x * (n >> 3) + min(x, n & 7) + (blockIdx.x >> 3);
 }
 
@@ -281,7 +281,7 @@ __device__ __forceinline__ WaPlace wa_place(const WaArgs& a, int gw) {
   WaPlace w;
   const int rw = 4 / gw, rows = 32 * rw, wave = wa_wave();
   const int blocks = (a.N + rows - 1) / rows, hb = a.H / gw;
-  const int id = wa_block(), u = id / blocks;
+  const int id = wa_block(gridDim.x), u = id / blocks;
   // last rows first: in a short sequence they have the most keys
   const int blk = blocks - 1 - (id - u * blocks);
   w.b = u / hb;
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
 // The first tile of rows that see none of keys k0..k0+127 by the window.
 __device__ __forceinline__ int wa_behind(const WaArgs& a, int k0, int len) {
   const int64_t end = (int64_t)k0 + WA_KB - 1 + a.window;
-  // without rows for the other kernel the last tile is the sequence's
+  // where no blocks take the rest the last tile is the sequence's
   if (a.slots == 0 && k0 < a.sinks) return (len + WA_T - 1) / WA_T;
   return (int)((min(end, (int64_t)len) + WA_T - 1) / WA_T);
 }
@@ -633,14 +633,21 @@ k_wa_dkv(const WaArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = wa_wave(), part = PARTS == 1 ? 0 : wave >> 2;
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
-  const int id = wa_block() / a.split, share = wa_block() - id * a.split;
-  const int u = id / nkb, k0 = (id - u * nkb) * WA_KB;
+  const int main = a.B * a.KV * nkb * a.split;
+  // behind: this block takes rows behind the window of first tokens
+  const bool behind = (int)blockIdx.x >= main;
+  const int shares = behind ? a.slots : a.split;
+  const int at = behind ? (int)blockIdx.x - main : wa_block(main);
+  const int id = at / shares, share = at - id * shares;
+  const int nb = behind ? (a.strips + 3) / 4 : nkb;
+  const int u = id / nb, k0 = (id - u * nb) * WA_KB;
   const int b = u / a.KV, kv = u - b * a.KV, G = a.H / a.KV;
   const int len = wa_len(a, b);
-  // the rows, in tiles, of each head: the window's
-  const int t0 = k0 / WA_T, total = max(wa_behind(a, k0, len) - t0, 0);
+  // the rows, in tiles, of each head
+  const int edge = wa_behind(a, k0, len), t0 = behind ? edge : k0 / WA_T;
+  const int total = max((behind ? (len + WA_T - 1) / WA_T : edge) - t0, 0);
   // (head, tile) pairs: this block's share of them
-  const int each = (total * G + a.split - 1) / a.split;
+  const int each = (total * G + shares - 1) / shares;
   const int it0 = min(share * each, total * G), it1 = min(it0 + each, total * G);
   const int wk = k0 + (wave & 3) * 32;   // this wave's first key
   const int key = wk + col;
@@ -649,9 +656,9 @@ k_wa_dkv(const WaArgs a) {
   for (int t = 0; t < DT; ++t) ak[t] = av[t] = (wa_f16)(0.0f);
   if (it0 < it1) {
     wa_bf8 kf[D / 16], vf[D / 16];
-    const int at = min(key, len - 1);
-    wa_row<D>(a.k.p + b * a.k.sB + kv * a.k.sH + at * a.k.sN, half, kf);
-    wa_row<D>(a.v.p + b * a.v.sB + kv * a.v.sH + at * a.v.sN, half, vf);
+    const int kr = min(key, len - 1);
+    wa_row<D>(a.k.p + b * a.k.sB + kv * a.k.sH + kr * a.k.sN, half, kf);
+    wa_row<D>(a.v.p + b * a.v.sB + kv * a.v.sH + kr * a.v.sN, half, vf);
     // addresses of this wave's rows of the tile and of the other's
     const int own = part * 32 * D * 2, far = (part ^ (PARTS - 1)) * 32 * D * 2;
     const WaRows<D> rows(lane, own);
@@ -772,7 +779,7 @@ k_wa_dkv(const WaArgs a) {
       if (it + 1 < it1) step(it + 1, lds + BUF, lds);
     }
   }
-  if (a.split > 1) {
+  if (!behind && a.split > 1) {
     float* p = wa_split<D>(a, u, nkb, k0 / WA_KB, share) + (key - k0) * D + part * H2;
     wa_store_part<DT>(p, ak, half);
     wa_store_part<DT>(p + WA_KB * D, av, half);
@@ -780,103 +787,15 @@ k_wa_dkv(const WaArgs a) {
   }
   const bool split = a.slots > 0 && key < a.sinks;
   if (split) {
-    float* p = wa_part<D>(a, u, key / 32, 0) + (key % 32) * D + part * H2;
+    float* p = wa_part<D>(a, u, key / 32, behind ? 1 + share : 0) + (key % 32) * D + part * H2;
     wa_store_part<DT>(p, ak, half);
     wa_store_part<DT>(p + 32 * D, av, half);
   }
+  if (behind) return;
   const bool write = key < a.N && !split;
   const int64_t off = (((int64_t)b * a.N + key) * a.KV + kv) * D + part * H2;
   wa_store<H2>(a.dk + off, ak, a.scale, half, write);
   wa_store<H2>(a.dv + off, av, 1.0f, half, write);
-}
-
-// dK and dV of a strip of first tokens by rows behind the window: every row
-// sees all of them.  A wave works alone, on 32 rows at a time: rows come from
-// memory as operands and pass through the wave's own LDS for the transposed
-// ones; the next rows travel meanwhile.
-template <int D>
-__global__ void __launch_bounds__(WA_BLOCK, D == 64 ? 2 : 1) k_wa_sink(const WaArgs a) {
-  constexpr int TILE = 32 * D * 2, OWN = 2 * TILE + 2 * 32 * 4;
-  __shared__ __attribute__((aligned(16))) char all[4 * OWN];
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-  const int wave = wa_wave(), blocks = a.slots / 4;
-  const int us = blockIdx.x / blocks;
-  const int slot = (blockIdx.x - us * blocks) * 4 + wave;
-  const int u = us / a.strips, strip = us - u * a.strips;
-  const int b = u / a.KV, kv = u - b * a.KV, G = a.H / a.KV;
-  const int len = wa_len(a, b), key = strip * 32 + col;
-  char* tq = all + wave * OWN;
-  char* tg = tq + TILE;
-  float* stat = (float*)(tg + TILE);
-  // rows, in strips of 32, of each head
-  const int r0 = wa_behind(a, strip * 32 / WA_KB * WA_KB, len) * WA_T;
-  const int total = max((len - r0 + 31) / 32, 0), all_it = total * G;
-  const int each = (all_it + a.slots - 1) / a.slots;
-  const int it0 = min(slot * each, all_it), it1 = min(it0 + each, all_it);
-  wa_f16 ak[D / 32], av[D / 32];
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = (wa_f16)(0.0f);
-  if (it0 < it1) {
-    wa_bf8 kf[D / 16], vf[D / 16], qn[D / 16], gn[D / 16];
-    const int at = min(key, len - 1);
-    wa_row<D>(a.k.p + b * a.k.sB + kv * a.k.sH + at * a.k.sN, half, kf);
-    wa_row<D>(a.v.p + b * a.v.sB + kv * a.v.sH + at * a.v.sN, half, vf);
-    const WaRows<D> rows(lane);
-    const WaCols<D> cols(lane);
-    const float c = a.scale * WA_LOG2E;
-    float sn = 0.0f;  // lanes 0..31: lse, the others: delta
-    int head = kv * G + it0 / total, tile = it0 % total;
-    auto load = [&]() {
-      const int row = r0 + tile * 32 + col, in = min(row, len - 1);
-      wa_row<D>(a.q.p + b * a.q.sB + head * a.q.sH + in * a.q.sN, half, qn);
-      wa_row<D>(a.go.p + b * a.go.sB + head * a.go.sH + in * a.go.sN, half, gn);
-      const int64_t i = ((int64_t)b * a.H + head) * a.N + in;
-      sn = half ? a.delta[i] : row < len ? a.lse[i] : INFINITY;
-      if (++tile == total) {
-        tile = 0;
-        ++head;
-      }
-    };
-    load();
-    for (int it = it0; it < it1; ++it) {
-      wa_f16 s = (wa_f16)(0.0f), p = (wa_f16)(0.0f);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        *(wa_bf8*)(tq + rows.at[kk]) = qn[kk];
-        *(wa_bf8*)(tg + rows.at[kk]) = gn[kk];
-        s = wa_mfma(qn[kk], kf[kk], s);
-        p = wa_mfma(gn[kk], vf[kk], p);
-      }
-      stat[lane] = sn;
-      if (it + 1 < it1) load();
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const float4 ls = *(const float4*)(stat + 8 * r4 + 4 * half);
-        const float4 de = *(const float4*)(stat + 32 + 8 * r4 + 4 * half);
-        const float lj[4] = {ls.x, ls.y, ls.z, ls.w}, dj[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e = wa_exp2(fmaf(s[4 * r4 + j], c, -lj[j]));
-          s[4 * r4 + j] = e;
-          p[4 * r4 + j] = e * (p[4 * r4 + j] - dj[j]);
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const wa_bf8 pf = wa_operand(s, ks), df = wa_operand(p, ks);
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) {
-          av[t] = wa_mfma(cols.get(tg, ks, t), pf, av[t]);
-          ak[t] = wa_mfma(cols.get(tq, ks, t), df, ak[t]);
-        }
-      }
-    }
-  }
-  if (key < a.sinks) {  // the strip's other keys saw weights that are not theirs
-    float* p = wa_part<D>(a, u, strip, 1 + slot) + col * D;
-    wa_store_part<D / 32>(p, ak, half);
-    wa_store_part<D / 32>(p + 32 * D, av, half);
-  }
 }
 
 // dK and dV from parts, in fixed order.  The first blocks take a first token
@@ -938,15 +857,14 @@ __global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a) {
 
 // ---------------------------------------------------------------------------
 
-// Waves that share the rows behind the window of a strip of first tokens: at
-// least 128 rows each, 1024 waves in all.  0: there are no such rows.
+// Blocks that share the rows behind the window of 128 first tokens: at least
+// four (head, tile) pairs each, 512 blocks in all.  0: there are no such rows.
 static int wa_slots(int64_t U, int64_t G, int64_t N, int64_t window, int64_t sinks) {
   if (sinks <= 0 || N <= window) return 0;
-  const int64_t strips = (sinks + 31) / 32;
-  int64_t n = G * ((N - window + 31) / 32) / 4;
-  const int64_t most = 1024 / (U * strips);
+  int64_t n = G * ((N - window + WA_T - 1) / WA_T) / 4;
+  const int64_t most = 512 / (U * ((sinks + WA_KB - 1) / WA_KB));
   if (n > most) n = most;
-  return (int)((n < 4 ? 4 : n) / 4 * 4);
+  return (int)(n < 1 ? 1 : n);
 }
 
 // Blocks that share the rows of 128 keys where there are fewer of those than
@@ -1040,16 +958,15 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
   const int gw = wa_heads_a_block(H / KV);
   const int64_t grid = wa_row_grid(B, H, N, gw);
   a.splits = part + wa_slot_floats(B * KV, D, a.sinks, a.slots);
-  const int64_t kgrid = B * KV * ((N + WA_KB - 1) / WA_KB) * a.split;
-  const int64_t sgrid = B * KV * a.strips * (a.slots / 4);
+  const int64_t kgrid = B * KV * (((N + WA_KB - 1) / WA_KB) * a.split +
+                                  (a.strips + 3) / 4 * a.slots);
   // blocks that add parts: see k_wa_sum
   const int64_t first = a.slots ? a.sinks : 0;
   const int64_t sums = first + (a.split > 1 ? (N - first + 4096 / D - 1) / (4096 / D) : 0);
-  if (grid > 0x7fffffff || kgrid > 0x7fffffff || sgrid > 0x7fffffff ||
-      B * KV > 65535 || (D != 64 && D != 128))
+  if (grid > 0x7fffffff || kgrid > 0x7fffffff || B * KV > 65535 || (D != 64 && D != 128))
     return 9003;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 rows((unsigned)grid), keys((unsigned)kgrid), strips((unsigned)sgrid);
+  const dim3 rows((unsigned)grid), keys((unsigned)kgrid);
   const dim3 adds((unsigned)sums, (unsigned)(B * KV));
   if (D == 64) {
     hipLaunchKernelGGL((k_wa_dq<64>), rows, dim3(WA_BLOCK), 0, s, a, gw);
@@ -1060,12 +977,10 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
       hipLaunchKernelGGL((k_wa_dkv<64, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
     else
       hipLaunchKernelGGL((k_wa_dkv<64, 1>), keys, dim3(WA_BLOCK), 0, s, a);
-    if (a.slots) hipLaunchKernelGGL((k_wa_sink<64>), strips, dim3(WA_BLOCK), 0, s, a);
     if (sums) hipLaunchKernelGGL((k_wa_sum<64>), adds, dim3(1024), 0, s, a);
   } else {
     hipLaunchKernelGGL((k_wa_dq<128>), rows, dim3(WA_BLOCK), 0, s, a, gw);
     hipLaunchKernelGGL((k_wa_dkv<128, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
-    if (a.slots) hipLaunchKernelGGL((k_wa_sink<128>), strips, dim3(WA_BLOCK), 0, s, a);
     if (sums) hipLaunchKernelGGL((k_wa_sum<128>), adds, dim3(1024), 0, s, a);
   }
   return (int)hipGetLastError();
