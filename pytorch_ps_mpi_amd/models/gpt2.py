@@ -33,7 +33,7 @@ class CausalBlock(nn.Module):
         self.local = not (window is None and kv_heads is None
                           and rotary is None)
         self.window, self.sinks = window, sinks
-        self.kv_heads = kv_heads or heads
+        self.kv_heads = heads if kv_heads is None else kv_heads
         self.rotary = rotary
         self.qkv = FusedLinear(
             dim, dim // heads * (heads + 2 * self.kv_heads))
@@ -57,9 +57,12 @@ class CausalBlock(nn.Module):
             q, k, v = self.qkv(h).view(B, T, -1, hd).split(
                 [self.heads, kv, kv], 2)
             if self.rotary is not None:
+                if pos is None:
+                    pos = torch.arange(T, device=h.device)[None]
                 q, k = self.rotary(q, k, pos)
             y = fused_window_sdpa(q.transpose(1, 2), k.transpose(1, 2),
-                                  v.transpose(1, 2), self.window or T,
+                                  v.transpose(1, 2),
+                                  T if self.window is None else self.window,
                                   self.sinks)
         return self.proj(y.transpose(1, 2).reshape(B, T, D))
 
@@ -89,9 +92,12 @@ class GPT2(nn.Module):
                  window=None, sinks=0, kv_heads=None, rotary=False,
                  layer_scale=None):
         super().__init__()
-        if dim % heads or heads % (kv_heads or heads):
+        if dim % heads or (kv_heads is not None and
+                           (kv_heads < 1 or heads % kv_heads)):
             raise ValueError("heads must divide dim, kv_heads must divide "
                              "heads")
+        if (window is not None and window < 1) or sinks < 0:
+            raise ValueError("window must be 1 or more, sinks 0 or more")
         self.wte = nn.Embedding(vocab, dim)
         rot = AxialRotary(dim // heads, (dim // heads // 2,)) if rotary \
             else None

@@ -213,6 +213,8 @@ def fused_adamw(p, m1, m2, g, p_out=None, *, lr, beta1=0.9, beta2=0.999,
         (offset + element index, seed, step) alone: a buffer updated in parts
         (``offset`` = where the part starts) rounds as it would in one.
         An infinity or NaN makes the values of its 256 elements read as NaN.
+    step : counts from 1; it enters as a number, so a captured graph repeats
+        the step that it was captured with.
     """
     n = p.numel()
     eight = isinstance(m1, State8)

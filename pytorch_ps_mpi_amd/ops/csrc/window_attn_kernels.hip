@@ -584,15 +584,6 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
 // ---------------------------------------------------------------------------
 // backward: dK and dV
 // ---------------------------------------------------------------------------
-// A block: 128 keys of a key head and the rows that see them by the window.
-//
-// Eight waves in pairs: wave w and w + 4 own the same 32 keys and lie on one
-// SIMD.  Each computes P and dS of its half of the tile's rows, hands them over
-// through LDS (as operands: each lane writes what the same lane of the other
-// reads) and sums dK and dV over all rows for its half of D.  Full sums in one
-// wave, with K and V in registers as well, left one wave a SIMD: 738 us where
-// this takes _US_ (8192 rows, 32 over 8 heads of 128, window 1024).
-
 // The first tile of rows that see none of keys k0..k0+127 by the window.
 __device__ __forceinline__ int wa_behind(const WaArgs& a, int k0, int len) {
   const int64_t end = (int64_t)k0 + WA_KB - 1 + a.window;
@@ -621,6 +612,16 @@ __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int h
       *(float4*)(row + 32 * t + 8 * r4 + 4 * half) = v;
     }
 }
+
+// A block: 128 keys of a key head and the rows that see them by the window.
+//
+// PARTS 2: eight waves in pairs; wave w and w + 4 own the same 32 keys and lie
+// on one SIMD.  Each computes P and dS of its half of the tile's rows, hands
+// them over through LDS (as operands: each lane writes what the same lane of
+// the other reads) and sums dK and dV over all rows for its half of D.  With
+// full sums in one wave, and K and V in registers as well, D = 128 leaves one
+// wave a SIMD: 738 us where pairs take 461 (8192 rows, 32 over 8 heads, window
+// 1024; 310 with what came later).  PARTS 1: a wave takes all rows and all of D.
 
 template <int D, int PARTS>
 __global__ void __launch_bounds__(PARTS * WA_BLOCK, PARTS == 1 ? 3 : 2)
@@ -806,10 +807,12 @@ __global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a) {
   constexpr int W = 1024 / D;
   __shared__ float lds[2][W][D];
   const int first = a.slots > 0 ? a.sinks : 0;  // keys with parts of strips
-  const int u = blockIdx.y, b = u / a.KV, kv = u - b * a.KV;
+  const int per = gridDim.x / (a.B * a.KV);
+  const int u = blockIdx.x / per, x = blockIdx.x - u * per;
+  const int b = u / a.KV, kv = u - b * a.KV;
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
-  if ((int)blockIdx.x >= first) {
-    const int key = first + ((int)blockIdx.x - first) * (4096 / D) + threadIdx.x / (D / 4);
+  if (x >= first) {
+    const int key = first + (x - first) * (4096 / D) + threadIdx.x / (D / 4);
     const int d = threadIdx.x % (D / 4) * 4;
     if (key >= a.N) return;
     const float* p = wa_split<D>(a, u, nkb, key / WA_KB, 0) + (key % WA_KB) * D + d;
@@ -826,7 +829,7 @@ __global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a) {
     *(uint2*)(a.dv + off) = ov;
     return;
   }
-  const int key = blockIdx.x, d = threadIdx.x % D, w = threadIdx.x / D;
+  const int key = x, d = threadIdx.x % D, w = threadIdx.x / D;
   float sk = 0.0f, sv = 0.0f;
   // part 0 is the rows' by the window, unless those are shared out themselves
   for (int s = w + (a.split > 1); s <= a.slots; s += W) {
@@ -869,7 +872,7 @@ static int wa_slots(int64_t U, int64_t G, int64_t N, int64_t window, int64_t sin
 
 // Blocks that share the rows of 128 keys where there are fewer of those than
 // CUs: one round of blocks, with at least four (head, tile) pairs each.  6 sequences of
-// 777, 8 over 2 heads of 128, window 100: 43 us in 84 blocks, _SPLIT_.
+// 777, 8 over 2 heads of 128, window 100: 43 us in 84 blocks, 26 in 252.
 static int wa_splits(int64_t U, int64_t G, int64_t N, int64_t window) {
   const int64_t blocks = U * ((N + WA_KB - 1) / WA_KB);
   const int64_t rows = window + WA_KB < N ? window + WA_KB : N;
@@ -962,12 +965,13 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
                                   (a.strips + 3) / 4 * a.slots);
   // blocks that add parts: see k_wa_sum
   const int64_t first = a.slots ? a.sinks : 0;
-  const int64_t sums = first + (a.split > 1 ? (N - first + 4096 / D - 1) / (4096 / D) : 0);
-  if (grid > 0x7fffffff || kgrid > 0x7fffffff || B * KV > 65535 || (D != 64 && D != 128))
+  const int64_t sums =
+      B * KV * (first + (a.split > 1 ? (N - first + 4096 / D - 1) / (4096 / D) : 0));
+  if (grid > 0x7fffffff || kgrid > 0x7fffffff || sums > 0x7fffffff || (D != 64 && D != 128))
     return 9003;
   hipStream_t s = (hipStream_t)stream;
   const dim3 rows((unsigned)grid), keys((unsigned)kgrid);
-  const dim3 adds((unsigned)sums, (unsigned)(B * KV));
+  const dim3 adds((unsigned)sums);
   if (D == 64) {
     hipLaunchKernelGGL((k_wa_dq<64>), rows, dim3(WA_BLOCK), 0, s, a, gw);
     // Pairs of waves where blocks do not fill the chip by themselves (16 key

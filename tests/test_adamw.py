@@ -181,3 +181,40 @@ def test_refusals():
         s8(n, True).values(torch.float16)
     with pytest.raises(ValueError):
         AdamW(models.build_model("mlp").named_parameters(), state_bits=4)
+
+
+def _worker(rank, port, mode, bits, out):
+    import os
+    os.environ.update(RANK=str(rank), WORLD_SIZE="2", LOCAL_RANK=str(rank),
+                      MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    import torch.distributed as dist
+    from pytorch_ps_mpi_amd import init_distributed
+    init_distributed(backend="gloo")
+    torch.manual_seed(0)
+    m = models.build_model("mlp")
+    o = AdamW(m.named_parameters(), lr=1e-3, state_bits=bits, mode=mode,
+              grad_scale="mean", bucket_mb=0.05,
+              no_decay=lambda n, p: p.dim() < 2)
+    _train(m, o, steps=4, seed=rank)
+    if mode != "async":
+        cs = [None, None]
+        dist.all_gather_object(cs, o.flat.param_checksum())
+        assert len(set(cs)) == 1
+    o.finish()
+    assert torch.isfinite(_flat(m)).all()
+    if rank == 0:
+        open(out, "w").write("ok")
+
+
+@pytest.mark.parametrize("mode,bits", [("replicated", 8), ("ps", 8),
+                                       ("async", 8), ("replicated", 32)])
+def test_two_ranks(tmp_path, mode, bits):
+    """Every exchange mode; ranks that update alike round alike."""
+    import socket
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    out = tmp_path / "ok"
+    mp.spawn(_worker, args=(port, mode, bits, str(out)), nprocs=2, join=True)
+    assert out.read_text() == "ok"

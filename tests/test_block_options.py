@@ -65,9 +65,18 @@ def test_window_limits_what_a_token_sees():
         assert (d[7:] > 0).all() if reaches else (d[7:] == 0).all()
 
 
-def test_refusal():
+@pytest.mark.parametrize("bad", [dict(kv_heads=3), dict(kv_heads=0),
+                                 dict(window=0), dict(sinks=-1)])
+def test_refusals(bad):
     with pytest.raises(ValueError):
-        _gpt(kv_heads=3)
+        _gpt(**bad)
+
+
+def test_block_alone_takes_positions_by_itself():
+    m = _gpt(layer_scale=None)
+    x = torch.randn(2, 9, 256)
+    pos = torch.arange(9)[None]
+    assert torch.equal(m.blocks[0](x), m.blocks[0](x, pos))
 
 
 def test_registry_passes_options():

@@ -103,6 +103,17 @@ def test_head_groups(H, KV):
     _check(*_make(2, H, KV, 150, 64, H), window=50, sinks=2)
 
 
+@pytest.mark.parametrize("B,H,KV,N,D,window,sinks", [
+    (4, 64, 64, 257, 64, 60, 5),      # key blocks for more than two rounds
+    (4, 64, 64, 257, 128, 60, 0),
+    (6, 32, 16, 300, 64, 50, 130),    # more than one round, first tokens
+    (1, 8, 1, 1500, 64, 100, 200),    # few key blocks: their rows shared out
+    (2, 6, 1, 700, 128, 90, 33),
+])
+def test_how_blocks_share_the_work(B, H, KV, N, D, window, sinks):
+    _check(*_make(B, H, KV, N, D, N), window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_padded_batches(D):
     """Lengths zero, one, odd, whole, and beyond the tensor; what stands behind
