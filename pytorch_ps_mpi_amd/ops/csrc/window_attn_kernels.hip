@@ -23,7 +23,7 @@
 //
 // Tiles of 64 rows stand in LDS row-major with their 16-byte granules swizzled
 // (wa_swz) so that neither the row reads nor the transposing reads meet in a
-// bank.  Tiles are double-buffered: the next one travels to registers while
+// bank.  Tiles are double-buffered: the next one travels to LDS directly while
 // this one is worked on; one barrier a tile.
 //
 // Four waves share a tile.  In the forward and dQ kernels they are up to four
@@ -34,6 +34,11 @@
 // The first tokens are seen by all rows: their dK/dV would be one block's work
 // of N rows among blocks of `window` rows.  The rows behind the window are
 // shared out over further blocks; a last kernel adds their parts in fixed order.
+//
+// Bound by the matrix instructions and the softmax arithmetic between them.
+// 8192 rows, 32 over 8 heads of 128, window 1024, 4 first tokens: forward 173
+// us (750 TFLOP/s of visible work), dQ 216, dK/dV 360, their sums 5.  8 x 1024
+// rows, 12 heads of 64, window 256: 25, 26, 44 and 4 us.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -621,7 +626,7 @@ __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int h
 // the other reads) and sums dK and dV over all rows for its half of D.  With
 // full sums in one wave, and K and V in registers as well, D = 128 leaves one
 // wave a SIMD: 738 us where pairs take 461 (8192 rows, 32 over 8 heads, window
-// 1024; 310 with what came later).  PARTS 1: a wave takes all rows and all of D.
+// 1024; 360 with what came later, the rows behind the window included).  PARTS 1: a wave takes all rows and all of D.
 
 template <int D, int PARTS>
 __global__ void __launch_bounds__(PARTS * WA_BLOCK, PARTS == 1 ? 3 : 2)
