@@ -161,6 +161,24 @@ class State8:
         return torch.where(c > top, -x, x).to(dtype)
 
 
+def _overlap(written, read):
+    """Whether a written tensor shares memory with another one."""
+    spans = []
+    for i, t in enumerate((*written, *read)):
+        start = t.data_ptr()
+        spans.append((start, start + t.numel() * t.element_size(),
+                      i < len(written)))
+    spans.sort()
+    end, end_written = 0, 0   # of all so far, of those that are written
+    for start, stop, w in spans:
+        if start < stop:
+            if start < (end if w else end_written):
+                return True
+            end = max(end, stop)
+            end_written = max(end_written, stop) if w else end_written
+    return False
+
+
 def _mix32(h):
     h = h ^ (h >> 16)
     h = (h * 0x7feb352d) & _MASK32
@@ -206,6 +224,7 @@ def fused_adamw(p, m1, m2, g, p_out=None, *, lr, beta1=0.9, beta2=0.999,
 
     p, g : flat fp32.  p_out : optional bf16/fp32 model copy.
     m1, m2 : both flat fp32, or both State8 (signed / unsigned).
+    None of p, p_out and the states may share memory with another tensor.
     decay : optional fp32 factor on ``wd`` for each 256 elements (tensors that
         start at multiples of 256 get their own; None decays everything).
     offset, seed : with 8-bit states a value between two codes is rounded up
@@ -263,6 +282,11 @@ def fused_adamw(p, m1, m2, g, p_out=None, *, lr, beta1=0.9, beta2=0.999,
                          lr / bc1, lr * wd, beta1, beta2, bc2 ** -0.5, eps,
                          gscale, key)
         return
+    written = [p] + ([m1.codes, m1.scales, m2.codes, m2.scales] if eight
+                     else [m1, m2]) + ([] if p_out is None else [p_out])
+    if _overlap(written, [g] if decay is None else [g, decay]):
+        raise ValueError("p, p_out and the states must not share memory with "
+                         "each other, g or decay")
     d = g * gscale
     m = beta1 * (m1.values() if eight else m1) + (1.0 - beta1) * d
     v = beta2 * (m2.values() if eight else m2) + (1.0 - beta2) * d * d

@@ -6,6 +6,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <cstdint>
+#include <iterator>
 #include <vector>
 
 extern "C" {
@@ -264,6 +265,19 @@ void fused_adamw(at::Tensor p, c10::optional<at::Tensor> p_out, at::Tensor g,
     out_ptr = p_out->data_ptr();
     kind = is_bf16(*p_out) ? 1 : 2;
   }
+  struct { const at::Tensor* t; bool written; } all[] = {
+      {&p, true}, {&m, true}, {&v, true}, {s8 ? &*ms : nullptr, true},
+      {s8 ? &*vs : nullptr, true}, {p_out ? &*p_out : nullptr, true},
+      {&g, false}, {decay ? &*decay : nullptr, false}};
+  for (const auto& a : all)
+    for (const auto* b = &a + 1; b < std::end(all); ++b) {
+      if (!a.t || !b->t || !(a.written || b->written)) continue;
+      const char *x = (const char*)a.t->data_ptr(), *y = (const char*)b->t->data_ptr();
+      // ValueError, as the CPU path raises
+      TORCH_CHECK_VALUE(x + a.t->nbytes() <= y || y + b->t->nbytes() <= x,
+                        "p, p_out and the states must not share memory with "
+                        "each other, g or decay");
+    }
   const c10::DeviceGuard guard(p.device());
   throw_on(ps_fused_adamw(cur_stream(p), p.data_ptr<float>(), out_ptr, kind,
                           g.data_ptr<float>(), m.data_ptr(), v.data_ptr(), msp,

@@ -143,6 +143,31 @@ def test_checkpoint_resume(tmp_path, bits):
     assert torch.equal(_flat(m3), before)
 
 
+def overlapping(dev):
+    """Calls of fused_adamw in which a written tensor shares memory."""
+    n = 512
+    t = lambda k=n: torch.zeros(k, device=dev)  # noqa: E731
+    a, b, c = t(), t(), t(3 * n)
+    e8, f8 = (ops.State8.zeros(n, s, dev) for s in (True, False))
+    bad = [
+        ((a, b, b, t()), {}), ((a, a, b, t()), {}), ((a, b, t(), a), {}),
+        ((a, b, t(), b), {}), ((a, b, t(), t()), dict(p_out=a)),
+        ((c[:n], c[256:256 + n], t(), t()), {}),
+        ((a, e8, ops.State8(e8.codes, t(2), False), t()), {}),
+        ((a, e8, ops.State8(f8.codes, e8.scales, False), t()), {}),
+        ((a, b, t(), t()), dict(decay=b[:2])),
+    ]
+    for args, kw in bad:
+        with pytest.raises(ValueError, match="share memory"):
+            ops.fused_adamw(*args, lr=1e-3, **kw)
+    # neighbours, and a gradient that holds the factors: fine
+    ops.fused_adamw(c[:n], c[n:2 * n], c[2 * n:], a, decay=a[:2], lr=1e-3)
+
+
+def test_shared_memory_is_refused():
+    overlapping("cpu")
+
+
 def test_refusals():
     n = 512
     t = lambda k=n: torch.zeros(k)  # noqa: E731

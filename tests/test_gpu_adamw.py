@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from pytorch_ps_mpi_amd import AdamW, models, ops
+from test_adamw import overlapping
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -191,3 +192,7 @@ def test_optimizer_trains_mlp_like_cpu(bits):
     # where a gradient is within rounding of zero its sign is not determined
     assert (got[0] - got[1]).abs().max() <= 2 * 3 * 3.2e-3
     assert (got[0] - got[1]).norm() <= 1e-2 * got[0].norm()
+
+
+def test_shared_memory_is_refused():
+    overlapping(DEV)
