@@ -34,6 +34,7 @@ struct RopeArgs {
   int64_t pA, pB, pN; // strides of pos
   int pos64;
   int64_t rows;       // B * N
+  int64_t first;      // first row of this launch
   int N, D, P;
   int start[4];       // first pair of axis 1, 2, 3 (P where there is none)
   float sign;         // -1: backward
@@ -101,7 +102,7 @@ template <typename T, bool INTER>
 __global__ void __launch_bounds__(RP_BLOCK) k_rope(const RopeArgs a) {
   extern __shared__ float2 cs[];
   constexpr int V = RpVec<T>::N;
-  const int64_t row0 = (int64_t)blockIdx.x * RP_TOK;
+  const int64_t row0 = a.first + (int64_t)blockIdx.x * RP_TOK;
   const int toks = (int)min((int64_t)RP_TOK, a.rows - row0);
   rp_angles(a, row0, toks, cs);
   __syncthreads();
@@ -156,13 +157,18 @@ __global__ void __launch_bounds__(RP_BLOCK) k_rope(const RopeArgs a) {
 }
 
 template <typename T>
-static void rp_launch(hipStream_t s, const RopeArgs& a, bool inter) {
-  const int grid = (int)((a.rows + RP_TOK - 1) / RP_TOK);
+static void rp_launch(hipStream_t s, RopeArgs a, bool inter) {
+  // a launch holds fewer than 2^32 threads: more rows take several
+  constexpr int64_t MOST = 1 << 23;
   const size_t lds = (size_t)RP_TOK * a.P * sizeof(float2);
-  if (inter)
-    hipLaunchKernelGGL((k_rope<T, true>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
-  else
-    hipLaunchKernelGGL((k_rope<T, false>), dim3(grid), dim3(RP_BLOCK), lds, s, a);
+  for (a.first = 0; a.first < a.rows; a.first += MOST * RP_TOK) {
+    const int64_t left = (a.rows - a.first + RP_TOK - 1) / RP_TOK;
+    const dim3 grid((unsigned)(left < MOST ? left : MOST));
+    if (inter)
+      hipLaunchKernelGGL((k_rope<T, true>), grid, dim3(RP_BLOCK), lds, s, a);
+    else
+      hipLaunchKernelGGL((k_rope<T, false>), grid, dim3(RP_BLOCK), lds, s, a);
+  }
 }
 
 // strides: q's B, N, H, k's B, N, H, pos's axis, B, N.  dtype: 0 bf16, 1 fp16,
@@ -175,7 +181,7 @@ extern "C" int ps_rope(void* stream, const void* q, const void* k, void* yq,
   const int64_t rows = B * N;
   if (rows <= 0) return 0;
   if (P < 1 || P > RP_MAXP || 2 * P > D ||
-      (rows + RP_TOK - 1) / RP_TOK > 0x7fffffff || N > 0x7fffffff ||
+      N > 0x7fffffff ||
       (int64_t)RP_TOK * ((int64_t)H + KV) * D > 0x7fffffff)
     return 9003;
   RopeArgs a;

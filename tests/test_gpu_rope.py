@@ -102,3 +102,21 @@ def test_graph_replays():
         torch.cuda.synchronize()
         want = rot(q, q, pos)
         assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+
+
+def test_more_rows_than_a_launch_holds():
+    """2^23 blocks of four tokens are one launch; the rest take another."""
+    N = 2 ** 25 + 7
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(1, N, 1, 2, generator=g, device=DEV).bfloat16()
+    pos = torch.randint(0, 2_000_000, (1, N), generator=g, device=DEV,
+                        dtype=torch.int32)
+    rot = AxialRotary(2, (1,))
+    y, _ = rot(x, x[:, :, :1], pos)
+    for part in (slice(0, 50), slice(2 ** 25 - 50, N)):
+        want = by_hand(x[:, part].cpu(), pos[:, None, part].cpu(), (1,), False,
+                       False)
+        err = (y[:, part].cpu().double() - want).abs()
+        assert (err <= _tol(want, torch.bfloat16)).all(), err.max()
+    assert torch.equal(y[:, 2 ** 24:], rot(x[:, 2 ** 24:], x[:, 2 ** 24:],
+                                           pos[:, 2 ** 24:])[0])
