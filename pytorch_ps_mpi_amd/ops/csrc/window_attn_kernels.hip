@@ -58,6 +58,7 @@ typedef __attribute__((address_space(1))) const void wa_mem;
 #define WA_BLOCK 256
 #define WA_T 64           // rows of a tile
 #define WA_KB 128         // keys of a dK/dV block
+#define WA_MOST (1LL << 32)  // threads of a launch stay under this
 #define WA_LOG2E 1.4426950408889634f
 
 struct WaTensor {
@@ -808,12 +809,12 @@ k_wa_dkv(const WaArgs a) {
 // each, 1024 / D parts at a time; the others, where blocks shared the rows of
 // 128 keys, 4096 / D of the remaining keys each.
 template <int D>
-__global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a) {
+__global__ void __launch_bounds__(1024) k_wa_sum(const WaArgs a, int per, int from) {
   constexpr int W = 1024 / D;
   __shared__ float lds[2][W][D];
   const int first = a.slots > 0 ? a.sinks : 0;  // keys with parts of strips
-  const int per = gridDim.x / (a.B * a.KV);
-  const int u = blockIdx.x / per, x = blockIdx.x - u * per;
+  const int id = from + blockIdx.x;  // `per` blocks a key head
+  const int u = id / per, x = id - u * per;
   const int b = u / a.KV, kv = u - b * a.KV;
   const int nkb = (a.N + WA_KB - 1) / WA_KB;
   if (x >= first) {
@@ -930,6 +931,16 @@ static int64_t wa_row_grid(int64_t B, int64_t H, int64_t N, int gw) {
   return B * (H / gw) * ((N + rows - 1) / rows);
 }
 
+// A launch holds fewer than 2^32 threads: more sums take several.
+template <int D>
+static void wa_sum(hipStream_t s, const WaArgs& a, int64_t sums) {
+  constexpr int64_t MOST = 1 << 21;
+  const int per = (int)(sums / ((int64_t)a.B * a.KV));
+  for (int64_t from = 0; from < sums; from += MOST)
+    hipLaunchKernelGGL((k_wa_sum<D>), dim3((unsigned)(sums - from < MOST ? sums - from : MOST)),
+                       dim3(1024), 0, s, a, per, (int)from);
+}
+
 // st: strides (B, H, N) of q, k, v, o, go; o is written as [B, N, H, D]
 extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
                          void* o, float* lse, const int32_t* lengths,
@@ -943,7 +954,7 @@ extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void*
   a.out = (__bf16*)o; a.lse = lse;
   const int gw = wa_heads_a_block(H / KV);
   const int64_t grid = wa_row_grid(B, H, N, gw);
-  if (grid > 0x7fffffff || (D != 64 && D != 128)) return 9003;
+  if (grid >= WA_MOST / WA_BLOCK || (D != 64 && D != 128)) return 9003;
   hipStream_t s = (hipStream_t)stream;
   if (D == 64) hipLaunchKernelGGL((k_wa_fwd<64>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
   else hipLaunchKernelGGL((k_wa_fwd<128>), dim3((unsigned)grid), dim3(WA_BLOCK), 0, s, a, gw);
@@ -972,11 +983,11 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
   const int64_t first = a.slots ? a.sinks : 0;
   const int64_t sums =
       B * KV * (first + (a.split > 1 ? (N - first + 4096 / D - 1) / (4096 / D) : 0));
-  if (grid > 0x7fffffff || kgrid > 0x7fffffff || sums > 0x7fffffff || (D != 64 && D != 128))
+  if (grid >= WA_MOST / WA_BLOCK || kgrid >= WA_MOST / (2 * WA_BLOCK) || sums > 0x7fffffff ||
+      (D != 64 && D != 128))
     return 9003;
   hipStream_t s = (hipStream_t)stream;
   const dim3 rows((unsigned)grid), keys((unsigned)kgrid);
-  const dim3 adds((unsigned)sums);
   if (D == 64) {
     hipLaunchKernelGGL((k_wa_dq<64>), rows, dim3(WA_BLOCK), 0, s, a, gw);
     // Pairs of waves where blocks do not fill the chip by themselves (16 key
@@ -986,11 +997,11 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
       hipLaunchKernelGGL((k_wa_dkv<64, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
     else
       hipLaunchKernelGGL((k_wa_dkv<64, 1>), keys, dim3(WA_BLOCK), 0, s, a);
-    if (sums) hipLaunchKernelGGL((k_wa_sum<64>), adds, dim3(1024), 0, s, a);
+    wa_sum<64>(s, a, sums);
   } else {
     hipLaunchKernelGGL((k_wa_dq<128>), rows, dim3(WA_BLOCK), 0, s, a, gw);
     hipLaunchKernelGGL((k_wa_dkv<128, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
-    if (sums) hipLaunchKernelGGL((k_wa_sum<128>), adds, dim3(1024), 0, s, a);
+    wa_sum<128>(s, a, sums);
   }
   return (int)hipGetLastError();
 }

@@ -244,3 +244,23 @@ def test_types_without_kernel_and_refusals():
     o = fused_window_sdpa(x, k, v, 9)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(o.sum(), x, create_graph=True)
+
+
+def test_more_first_tokens_than_a_launch_holds():
+    """Sums of 2^21 first tokens over all key heads are one launch; the last
+    heads' take another.  The first and the last heads against 64 bits."""
+    H, N, window, sinks = 520, 4100, 2, 4097
+    assert H * sinks > 2 ** 21
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v, go = (torch.randn(1, H, N, 64, generator=g, device=DEV).bfloat16()
+                   for _ in range(4))
+    x = [t.requires_grad_() for t in (q, k, v)]
+    o = fused_window_sdpa(*x, window, sinks)
+    got = (o.detach(), *torch.autograd.grad(o, x, go))
+    for h in (0, H - 1):
+        part = [t.detach()[:, h:h + 1].cpu() for t in (q, k, v, go)]
+        want = by_hand(*part, window, sinks, None, 0.125)
+        tol = _bounds(*part, window, sinks, None, 0.125, want)
+        for name, a, b, t in zip(("o", "dq", "dk", "dv"), got, want, tol):
+            err = (a[:, h:h + 1].cpu().double() - b).abs()
+            assert (err <= t + 1e-30).all(), (h, name, err.max())
