@@ -249,7 +249,6 @@ template <int EPT, int TPR, typename R>
 __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int slot,
                                         int lane, int sub, float* lds) {
   constexpr int RPB = JnBlock<TPR>::ROWS;
-  if (slot < 0) return;
   float* out = a.part + ((int64_t)blockIdx.x * a.slots + slot) * a.D;
   if (RPB == 1) {
 #pragma unroll
@@ -269,24 +268,70 @@ __device__ __forceinline__ void jn_part(const JoinArgs& a, const float* acc, int
   }
 }
 
+// A lane's sums over the rows of its block, in registers or in its own places
+// in LDS: 16 bytes a lane, so that a wave's accesses meet in no bank.  No other
+// lane looks at them: no barrier.
+template <int EPT, int TPR, bool LDS>
+struct JnAcc {
+  float r[LDS ? 1 : EPT];
+  float4* at;
+  static constexpr int BYTES = LDS ? EPT * TPR * 4 : 0;
+  __device__ __forceinline__ void clear(char* lds, int lane) {
+    at = (float4*)lds + lane;
+#pragma unroll
+    for (int j = 0; j < EPT; j += 4) {
+      if constexpr (LDS) at[j / 4 * TPR] = make_float4(0, 0, 0, 0);
+      else r[j] = r[j + 1] = r[j + 2] = r[j + 3] = 0.0f;
+    }
+  }
+  // sum j becomes f(j, sum j)
+  template <typename F> __device__ __forceinline__ void add(F f) {
+#pragma unroll
+    for (int j = 0; j < EPT; j += 4) {
+      if constexpr (LDS) {
+        float4 s = at[j / 4 * TPR];
+        s.x = f(j, s.x);
+        s.y = f(j + 1, s.y);
+        s.z = f(j + 2, s.z);
+        s.w = f(j + 3, s.w);
+        at[j / 4 * TPR] = s;
+      } else {
+#pragma unroll
+        for (int k = j; k < j + 4; ++k) r[k] = f(k, r[k]);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float* to) {
+    add([&](int j, float s) { return to[j] = s; });
+  }
+};
+
 template <typename T, int EPT, int TPR, bool POST, int GATE>
 __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) {
   using R = JnRow<T, EPT, TPR>;
   constexpr int RPB = JnBlock<TPR>::ROWS;
   __shared__ float2 red[2 * (TPR / 64)];
   __shared__ float lds[RPB == 1 ? 1 : RPB * EPT * TPR];
+  // Five sums of 16 elements do not fit beside a row of 512 lanes: with Post
+  // they went to scratch (4096 rows of 8192, a gate vector: 364 us, 126 so).
+  constexpr bool FAR = POST && EPT == 16 && TPR == 512;
+  using Near = JnAcc<EPT, TPR, false>;
+  using Acc = JnAcc<EPT, TPR, FAR>;
+  __shared__ __attribute__((aligned(16))) char sums[FAR ? (3 + (GATE == 1)) * Acc::BYTES : 16];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int group = blockIdx.x / a.nb, blk = blockIdx.x - group * a.nb;
   const int D = a.D;
   int turn = 0;
   R w, pw, pb, gate;
-  float aw[EPT], ab[EPT], ag[GATE == 1 ? EPT : 1], apw[POST ? EPT : 1], apb[POST ? EPT : 1];
-#pragma unroll
-  for (int j = 0; j < EPT; ++j) {
-    aw[j] = ab[j] = 0.0f;
-    if (GATE == 1) ag[j] = 0.0f;
-    if (POST) apw[j] = apb[j] = 0.0f;
+  Near aw;
+  Acc ab, ag, apw, apb;
+  aw.clear(nullptr, lane);
+  ab.clear(sums, lane);
+  if (POST) {
+    apw.clear(sums + Acc::BYTES, lane);
+    apb.clear(sums + 2 * Acc::BYTES, lane);
   }
+  if (GATE == 1) ag.clear(sums + 3 * Acc::BYTES, lane);
   w.load(a.w, 0, lane, D);
   if (POST) {
     pw.load(a.pw, 0, lane, D);
@@ -331,12 +376,12 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
       if (GATE) n *= gate.get(j);
       const float xh = (fmaf(a.scale, x.get(j), n) - m1) * r1, g = dh.get(j);
       y[j] = xh;
-      aw[j] = fmaf(g, xh, aw[j]);
-      ab[j] += g;
       t[j] = g * w.get(j);
       s1 += t[j];
       s2 = fmaf(t[j], xh, s2);
     }
+    aw.add([&](int j, float s) { return fmaf(dh.get(j), y[j], s); });
+    ab.add([&](int j, float s) { return s + dh.get(j); });
     float2 s = jn_sum2<TPR>(s1, s2, red, turn);
     float c1 = a.layer ? s.x * a.invD : 0.0f, c2 = s.y * a.invD;
 #pragma unroll
@@ -346,21 +391,26 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
     }
     x.store(a.dx, off, lane, D);
     s1 = s2 = 0.0f;
+    auto uh = [&](int j) { return POST ? (u.get(j) - m2) * r2 : u.get(j); };
+    auto dg = [&](int j) {
+      return t[j] * (POST ? fmaf(uh(j), pw.get(j), pb.get(j)) : uh(j));
+    };
+    if (GATE == 1) ag.add([&](int j, float s) { return s + dg(j); });
+    if (GATE) {
 #pragma unroll
-    for (int j = 0; j < EPT; ++j) {
-      const float uh = POST ? (u.get(j) - m2) * r2 : u.get(j);
-      if (GATE) {
-        const float g = t[j] * (POST ? fmaf(uh, pw.get(j), pb.get(j)) : uh);
-        if (GATE == 1) ag[j] += g;
-        if (GATE == 2) dy.set(j, g);
+      for (int j = 0; j < EPT; ++j) {
+        if (GATE == 2) dy.set(j, dg(j));
         t[j] *= gate.get(j);
       }
-      if (POST) {
-        apw[j] = fmaf(t[j], uh, apw[j]);
-        apb[j] += t[j];
+    }
+    if (POST) {
+      apw.add([&](int j, float s) { return fmaf(t[j], uh(j), s); });
+      apb.add([&](int j, float s) { return s + t[j]; });
+#pragma unroll
+      for (int j = 0; j < EPT; ++j) {
         t[j] *= pw.get(j);
         s1 += t[j];
-        s2 = fmaf(t[j], uh, s2);
+        s2 = fmaf(t[j], uh(j), s2);
       }
     }
     if (GATE == 2 && a.dgate) dy.store(a.dgate, off, lane, D);
@@ -376,12 +426,18 @@ __global__ void __launch_bounds__(JnBlock<TPR>::N) k_join_bwd(const JoinArgs a) 
     u.store(a.du, off, lane, D);
   }
   // lanes past the row's end held w = pw = 0 and are not written
-  jn_part<EPT, TPR, R>(a, aw, a.slot_w, lane, sub, lds);
-  jn_part<EPT, TPR, R>(a, ab, a.slot_b, lane, sub, lds);
-  if (GATE == 1) jn_part<EPT, TPR, R>(a, ag, a.slot_g, lane, sub, lds);
+  auto part = [&](auto& acc, int slot) {
+    if (slot < 0) return;
+    float f[EPT];
+    acc.get(f);
+    jn_part<EPT, TPR, R>(a, f, slot, lane, sub, lds);
+  };
+  part(aw, a.slot_w);
+  part(ab, a.slot_b);
+  if (GATE == 1) part(ag, a.slot_g);
   if (POST) {
-    jn_part<EPT, TPR, R>(a, apw, a.slot_pw, lane, sub, lds);
-    jn_part<EPT, TPR, R>(a, apb, a.slot_pb, lane, sub, lds);
+    part(apw, a.slot_pw);
+    part(apb, a.slot_pb);
   }
 }
 

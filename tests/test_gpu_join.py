@@ -225,3 +225,12 @@ def test_empty_and_refusals():
     big = inputs(1, 1, 8200, torch.float32, "none", False, False)
     with pytest.raises(ValueError):
         call({n: None if v is None else v.to(DEV) for n, v in big.items()})
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "token"])
+def test_longest_rows_over_several_rows_a_block(dtype, gate):
+    """Rows past 4096 with both norms keep their sums in LDS; 256 blocks take
+    these rows, three or two each."""
+    B, T = (2, 300) if gate == "sample" else (1, 600)
+    _check(inputs(B, T, 5000, dtype, gate, True, True), 0.9, "layer")
