@@ -538,11 +538,16 @@ static void jn_pick(hipStream_t s, int grid, const JoinArgs& a) {
 // Blocks of a group: the backward kernel's registers let 2048 waves be on the
 // chip at once; more would only write more parts.  Forward 4096 waves: each
 // reads the weights once (49152 rows of 768: 62 us with 8192, 58 with 4096).
-static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool lean, bool backward) {
+// Rows of 256 lanes with Post wait at more barriers and want 8192 (8192 rows of
+// 4096: 59 us with 4096, 55 with 8192; 16384 of 1536: 54 and 48), without Post
+// or with 512 lanes they do not (16384 of 2048: 53 and 54; 4096 of 8192 with
+// Post: 61 and 65).
+static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool lean, bool post,
+                         bool backward) {
   const JnShape h = jn_shape(D, lean && backward);
   const int64_t rpb = h.tpr < 128 ? 256 / h.tpr : 1;
   const int64_t waves = h.tpr < 128 ? 4 : h.tpr / 64;
-  const int64_t most = (backward ? 2048 : 4096) / waves / groups;
+  const int64_t most = (backward ? 2048 : post && h.tpr == 256 ? 8192 : 4096) / waves / groups;
   int64_t nb = (rows + rpb - 1) / rpb;
   if (nb > most) nb = most;
   return nb < 1 ? 1 : nb;
@@ -550,7 +555,7 @@ static int64_t jn_blocks(int64_t groups, int64_t rows, int64_t D, bool lean, boo
 
 extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int post,
                                   int bf16) {
-  return jn_blocks(groups, rows, D, post || !bf16, true);
+  return jn_blocks(groups, rows, D, post || !bf16, post, true);
 }
 
 static int jn_check(const JoinArgs& a, int64_t groups) {
@@ -571,7 +576,7 @@ extern "C" int ps_join_fwd(void* stream, void* const* t, float* const* stats,
   a.my = stats[0]; a.ry = stats[1]; a.mu = stats[2]; a.ru = stats[3];
   a.rows = rows; a.D = (int)D; a.layer = layer; a.gate_kind = gate_kind;
   a.gate_step = gate_step; a.scale = scale; a.eps = eps; a.invD = 1.0f / (float)D;
-  a.nb = (int)jn_blocks(groups, rows, D, false, false);
+  a.nb = (int)jn_blocks(groups, rows, D, false, a.pw != nullptr, false);
   if (int e = jn_check(a, groups)) return e;
   const int grid = (int)(groups * a.nb);
   if (bf16) jn_pick<__hip_bfloat16, false>((hipStream_t)stream, grid, a);
