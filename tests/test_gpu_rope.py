@@ -120,3 +120,38 @@ def test_more_rows_than_a_launch_holds():
         assert (err <= _tol(want, torch.bfloat16)).all(), err.max()
     assert torch.equal(y[:, 2 ** 24:], rot(x[:, 2 ** 24:], x[:, 2 ** 24:],
                                            pos[:, 2 ** 24:])[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,sections", [
+    (96, (10, 6, 9)), (96, (43,)), (96, (20, 12, 12)), (64, (6, 4)),
+    (64, (30,)), (64, (3,)), (128, (17, 10, 15)), (20, (8,)), (17, (8,)),
+    (33, (5, 6)), (9, (4,)), (7, (1, 1)), (30, (15,)), (22, (9,)),
+])
+def test_ranges_that_vectors_do_not_divide(dtype, interleaved, D, sections):
+    """What turns and what passes through end anywhere; the latter keeps its
+    bits, NaN included, and results repeat."""
+    g = torch.Generator().manual_seed(D)
+    q, k = (torch.randn(2, 9, h, D, generator=g).clamp(-6, 6).to(dtype)
+            for h in (5, 2))
+    P = sum(sections)
+    if 2 * P < D:
+        q[:, ::2, :, 2 * P:] = float("nan")
+        q[:, 1::2, :, -1] = float("inf")
+    pos = torch.randint(0, 100_000, (len(sections), 2, 9), generator=g)
+    rot = AxialRotary(D, sections, interleaved=interleaved)
+    args = (q.to(DEV), k.to(DEV), pos.to(DEV))
+    y = rot(*args)
+    for got, x in zip(y, (q, k)):
+        got = got.cpu()
+        if 2 * P < D:
+            bits = torch.int16 if dtype == torch.bfloat16 else torch.int32
+            assert torch.equal(got[..., 2 * P:].contiguous().view(bits),
+                               x[..., 2 * P:].contiguous().view(bits))
+        want = by_hand(x, pos, sections, False, interleaved)[..., :2 * P]
+        err = (got[..., :2 * P].double() - want).abs()
+        assert (err <= _tol(want, dtype)).all(), err.max()
+    for _ in range(3):
+        for a, b in zip(rot(*args), y):
+            assert torch.equal(a.nan_to_num(), b.nan_to_num())
