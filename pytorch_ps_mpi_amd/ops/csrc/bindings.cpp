@@ -40,12 +40,12 @@ int ps_join_bwd(void* stream, void* const* t, float* const* stats,
 int64_t ps_wa_part_floats(int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
                           int64_t window, int64_t sinks);
 int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
-              void* o, float* lse, const int32_t* lengths, const int64_t* st,
-              int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
+              void* o, void* low, float* lse, const int32_t* lengths,
+              const int64_t* st, int64_t B, int64_t H, int64_t KV, int64_t N, int64_t D,
               int64_t window, int64_t sinks, float scale);
 int ps_wa_bwd(void* stream, const void* q, const void* k, const void* v,
-              const void* o, const void* go, float* lse, float* delta,
-              void* dq, void* dk, void* dv, float* part,
+              const void* o, const void* low, const void* go, float* lse,
+              float* delta, void* dq, void* dk, void* dv, float* part,
               const int32_t* lengths, const int64_t* st, int64_t B, int64_t H,
               int64_t KV, int64_t N, int64_t D, int64_t window, int64_t sinks,
               float scale);
@@ -1027,7 +1027,7 @@ static void wa_stat(const at::Tensor& t, const at::Tensor& q) {
 }
 
 void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
-            at::Tensor lse, c10::optional<at::Tensor> lengths, int64_t window,
+            c10::optional<at::Tensor> low, at::Tensor lse, c10::optional<at::Tensor> lengths, int64_t window,
             int64_t sinks, double scale) {
   int64_t st[15] = {0};
   TORCH_CHECK(k.dim() == 4 && q.dim() == 4, "q, k must be 4-D");
@@ -1035,18 +1035,20 @@ void wa_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
   wa_check(k, "k", q, k.size(1), st + 3);
   wa_check(v, "v", q, k.size(1), st + 6);
   wa_out(o, "o", q, q.size(1));
+  if (low) wa_out(*low, "low", q, q.size(1));
   wa_stat(lse, q);
   const int32_t* len = wa_lengths(lengths, q);
   const c10::DeviceGuard guard(q.device());
   throw_on(ps_wa_fwd(cur_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     o.data_ptr(), lse.data_ptr<float>(), len, st, q.size(0),
+                     o.data_ptr(), low ? low->data_ptr() : nullptr,
+                     lse.data_ptr<float>(), len, st, q.size(0),
                      q.size(1), k.size(1), q.size(2), q.size(3), window, sinks,
                      (float)scale),
            "wa_fwd");
 }
 
 void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
-            at::Tensor go, at::Tensor lse, at::Tensor delta, at::Tensor dq,
+            at::Tensor low, at::Tensor go, at::Tensor lse, at::Tensor delta, at::Tensor dq,
             at::Tensor dk, at::Tensor dv, at::Tensor part,
             c10::optional<at::Tensor> lengths, int64_t window, int64_t sinks,
             double scale) {
@@ -1056,6 +1058,7 @@ void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
   wa_check(k, "k", q, k.size(1), st + 3);
   wa_check(v, "v", q, k.size(1), st + 6);
   wa_check(o, "o", q, q.size(1), st + 9);
+  wa_out(low, "low", q, q.size(1));
   wa_check(go, "dout", q, q.size(1), st + 12);
   wa_out(dq, "dq", q, q.size(1));
   wa_out(dk, "dk", q, k.size(1));
@@ -1071,7 +1074,8 @@ void wa_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
   const int32_t* len = wa_lengths(lengths, q);
   const c10::DeviceGuard guard(q.device());
   throw_on(ps_wa_bwd(cur_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     o.data_ptr(), go.data_ptr(), lse.data_ptr<float>(),
+                     o.data_ptr(), low.data_ptr(), go.data_ptr(),
+                     lse.data_ptr<float>(),
                      delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
                      dv.data_ptr(), part.data_ptr<float>(), len, st, q.size(0),
                      q.size(1), k.size(1), q.size(2), q.size(3), window, sinks,
@@ -1102,7 +1106,8 @@ struct WindowSdpa : torch::autograd::Function<WindowSdpa> {
                             const at::Tensor& q_, const at::Tensor& k_,
                             const at::Tensor& v_,
                             const c10::optional<at::Tensor>& lengths,
-                            int64_t window, int64_t sinks, double scale) {
+                            int64_t window, int64_t sinks, double scale,
+                            bool grad) {
     TORCH_CHECK(q_.is_cuda() && q_.dim() == 4 && k_.dim() == 4 &&
                     v_.dim() == 4, "q, k, v must be 4-D on GPU");
     const c10::DeviceGuard guard(q_.device());
@@ -1112,10 +1117,12 @@ struct WindowSdpa : torch::autograd::Function<WindowSdpa> {
                          q.options().dtype(at::kFloat));
     const at::Tensor len = lengths.has_value() ? lengths->contiguous()
                                                : at::Tensor();
-    wa_fwd(q, k, v, o, lse, len.defined() ? c10::optional<at::Tensor>(len)
+    c10::optional<at::Tensor> low;
+    if (grad) low = wa_empty(q.size(0), q.size(1), q.size(2), q.size(3), q);
+    wa_fwd(q, k, v, o, low, lse, len.defined() ? c10::optional<at::Tensor>(len)
                                           : c10::optional<at::Tensor>(),
            window, sinks, scale);
-    ctx->save_for_backward({q, k, v, o, lse, len});
+    ctx->save_for_backward({q, k, v, o, lse, len, low ? *low : at::Tensor()});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
@@ -1137,12 +1144,12 @@ struct WindowSdpa : torch::autograd::Function<WindowSdpa> {
     auto delta = at::empty_like(s[4]);
     auto part = at::empty({ps_wa_part_floats(B, H, KV, N, D, window, sinks)},
                           q.options().dtype(at::kFloat));
-    wa_bwd(q, k, s[2], s[3], wa_rows16(g[0]), s[4], delta, dq, dk, dv, part,
+    wa_bwd(q, k, s[2], s[3], s[6], wa_rows16(g[0]), s[4], delta, dq, dk, dv, part,
            s[5].defined() ? c10::optional<at::Tensor>(s[5])
                           : c10::optional<at::Tensor>(),
            window, sinks, ctx->saved_data["scale"].toDouble());
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+            at::Tensor(), at::Tensor()};
   }
 };
 
@@ -1150,7 +1157,9 @@ static at::Tensor window_sdpa(at::Tensor q, at::Tensor k, at::Tensor v,
                               int64_t window, int64_t sinks,
                               c10::optional<at::Tensor> lengths,
                               double scale) {
-  return WindowSdpa::apply(q, k, v, lengths, window, sinks, scale);
+  const bool grad = at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  return WindowSdpa::apply(q, k, v, lengths, window, sinks, scale, grad);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

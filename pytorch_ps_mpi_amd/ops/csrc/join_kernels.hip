@@ -18,7 +18,7 @@
 // fixed order.  No atomics: results repeat bit for bit.
 //
 // bf16, 49152 rows of 768, one gate vector: forward 53 us (5.7 TB/s), backward
-// 115 (3.9 TB/s), sums 5.  8192 rows of 4096 with both norms: 52, 81 and 4 us.
+// 115 (3.9 TB/s), sums 5.  8192 rows of 4096 with both norms: 48, 77 and 4 us.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>

@@ -8,7 +8,11 @@
 //
 // q, k, v: bf16 of any strides with unit d stride, heads in groups that share
 // keys and values.  D is 64 or 128.  Scores, statistics and sums in fp32, P and
-// dS rounded to bf16 as operands of the matrix instructions.
+// dS rounded to bf16 as operands of the matrix instructions.  rowsum(dO * O)
+// takes O before its rounding (a second bf16 tensor holds the rest, written only
+// where a gradient will be asked for): what all values share cancels in dS, an
+// error of 2^-8 of it would not.  That costs 6 to 8 us of each pass at 8192 rows
+// of 32 heads of 128 and halves the error of dQ and dK where few keys are seen.
 //
 // Layout.  mfma 32x32x16: operand rows (or columns) are lane % 32, its
 // contraction index 8 * (lane / 32) + j; the result's column is lane % 32, its
@@ -36,9 +40,9 @@
 // shared out over further blocks; a last kernel adds their parts in fixed order.
 //
 // Bound by the matrix instructions and the softmax arithmetic between them.
-// 8192 rows, 32 over 8 heads of 128, window 1024, 4 first tokens: forward 173
-// us (750 TFLOP/s of visible work), dQ 216, dK/dV 360, their sums 5.  8 x 1024
-// rows, 12 heads of 64, window 256: 25, 26, 44 and 4 us.
+// 8192 rows, 32 over 8 heads of 128, window 1024, 4 first tokens: forward 182
+// us (710 TFLOP/s of visible work), dQ 222, dK/dV 350, their sums 5.  8 x 1024
+// rows, 12 heads of 64, window 256: 28, 29, 42 and 4 us.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -59,6 +63,8 @@ typedef __attribute__((address_space(1))) const void wa_mem;
 #define WA_T 64           // rows of a tile
 #define WA_KB 128         // keys of a dK/dV block
 #define WA_MOST (1LL << 32)  // threads of a launch stay under this
+// a call would put the accumulators into memory
+#define WA_INLINE __attribute__((always_inline))
 #define WA_LOG2E 1.4426950408889634f
 
 struct WaTensor {
@@ -69,6 +75,7 @@ struct WaTensor {
 struct WaArgs {
   WaTensor q, k, v, o, go;
   __bf16 *out, *dq, *dk, *dv;   // out, dq: [B,N,H,D]; dk, dv: [B,N,KV,D]
+  __bf16* low;                  // what out's rounding left out, as out; or null
   float *lse, *delta;           // [B,H,N]; lse of base 2
   float* part;                  // dK, dV parts of the first tokens
   const int32_t* lengths;       // [B], or null
@@ -229,23 +236,38 @@ struct WaCols {
   }
 };
 
-// Stores a transposed result (columns: 32 rows of the tensor, rows: D) times f,
-// 16 bytes a lane: the half waves swap so that each holds 8 neighbours.
+// 8 neighbours of a transposed result's row, 16 bytes a lane: the half waves
+// swap what they hold of them.
+__device__ __forceinline__ wa_u4 wa_eight(const uint32_t* u) {
+  auto a = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false);
+  auto b = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
+  return (wa_u4){a[0], b[0], a[1], b[1]};
+}
+
+// Stores a transposed result (columns: 32 rows of the tensor, rows: D) times f;
+// with `low` what the rounding left out as well.
 template <int D>
 __device__ __forceinline__ void wa_store(__bf16* row, const wa_f16* acc, float f,
-                                         int half, bool write) {
+                                         int half, bool write, __bf16* low = nullptr) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      uint32_t u[4];
+      uint32_t u[4], r[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        u[j] = wa_pack(acc[dt][8 * p + 2 * j] * f, acc[dt][8 * p + 2 * j + 1] * f);
-      auto a = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false);
-      auto b = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
-      const wa_u4 w = {a[0], b[0], a[1], b[1]};
-      if (write) *(wa_u4*)(row + 32 * dt + 16 * p + 8 * half) = w;
+      for (int j = 0; j < 4; ++j) {
+        const float x = acc[dt][8 * p + 2 * j] * f, y = acc[dt][8 * p + 2 * j + 1] * f;
+        u[j] = wa_pack(x, y);
+        r[j] = wa_pack(x - __uint_as_float(u[j] << 16),
+                       y - __uint_as_float(u[j] & 0xffff0000u));
+      }
+      const int at = 32 * dt + 16 * p + 8 * half;
+      const wa_u4 w = wa_eight(u);
+      if (write) *(wa_u4*)(row + at) = w;
+      if (low) {
+        const wa_u4 v = wa_eight(r);
+        if (write) *(wa_u4*)(low + at) = v;
+      }
     }
 }
 
@@ -373,14 +395,19 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
   mv.go(w.tile(0) * WA_T, w.len, ldv, wave);
   if (w.count > 1) mk.go(w.tile(1) * WA_T, w.len, ldk + TILE, wave);
   const float c = a.scale * WA_LOG2E;
-  float m = -3.0e38f, l = 0.0f;  // l: this half wave's keys
-  auto scores = [&](const char* tk, int sub, wa_f16& to) {
+  // This half wave's keys: the sum of the weights, for the statistic, and that of
+  // the weights as they are rounded for their product.  The output is divided
+  // by the latter: weights that add up to 1 leave a part that all values share
+  // as it is, and in dP - rowsum(dO * O) it cancels.
+  float m = -3.0e38f, l = 0.0f, lr = 0.0f;
+  const wa_bf2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+  auto scores = [&](const char* tk, int sub, wa_f16& to) WA_INLINE {
     to = (wa_f16)(0.0f);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) to = wa_mfma(rows.get(tk, sub, kk), qf[kk], to);
   };
   // scaled first: the products need no quieting before the comparisons
-  auto highest = [&](wa_f16& s) {
+  auto highest = [&](wa_f16& s) WA_INLINE {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 15; r += 2) top = fmaxf(fmaxf(top, s[r]), s[r + 1]);
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
   };
   // the strip's weights and their product; then the next strip's scores
   auto strip = [&](wa_f16& s, int seen, int k0, const char* tv, int sub, wa_f16& next,
-                   int seen_next, const char* tk, int sub_next) {
+                   int seen_next, const char* tk, int sub_next) WA_INLINE {
     float top = -INFINITY;
     if (seen == 2 && seen_next) {
       scores(tk, sub_next, next);
@@ -417,6 +444,7 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
     if (__any(mn > m + 8.0f)) {
       const float f = wa_exp2(m - mn);
       l *= f;
+      lr *= f;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) acc[t] *= f;
       m = mn;
@@ -429,6 +457,9 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
         l += s[r];
       }
       const wa_bf8 p = wa_operand(s, ks);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+        lr = __builtin_amdgcn_fdot2_f32_bf16((wa_bf2){p[j], p[j + 1]}, ones, lr, false);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
         acc[t] = wa_mfma(cols.get(tv, sub * 2 + ks, t), p, acc[t]);
@@ -445,17 +476,17 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
   // Nothing is read where the next tile arrives (`to`): the compiler need not
   // wait for it.
   auto first = [&](const char* __restrict__ tv, const char* __restrict__ tk,
-                   char* __restrict__ to, bool more, int n0, int k0, int seen1) {
+                   char* __restrict__ to, bool more, int n0, int k0, int seen1) WA_INLINE {
     if (more) mv.go(n0, w.len, to, wave);
     strip(s0, seen0, k0, tv, 0, s1, seen1, tk, 1);
   };
   auto second = [&](const char* __restrict__ tv, const char* __restrict__ tk,
-                    char* __restrict__ to, bool more, int n0, int k0, int seen1, int seen2) {
+                    char* __restrict__ to, bool more, int n0, int k0, int seen1, int seen2) WA_INLINE {
     if (more) mk.go(n0, w.len, to, wave);
     strip(s1, seen1, k0, tv, 1, s0, seen2, tk, 0);
   };
   // o: 0 or TILE, where this tile stands
-  auto step = [&](int it, int o) {
+  auto step = [&](int it, int o) WA_INLINE {
     const int k0 = w.tile(it) * WA_T;
     const bool more = it + 1 < w.count, more2 = it + 2 < w.count;
     const int n0 = more ? w.tile(it + 1) * WA_T : 0;
@@ -473,8 +504,9 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_fwd(const WaArgs a, int gw) 
     if (it + 1 < w.count) step(it + 1, TILE);
   }
   l = wa_other_sum(l);
+  lr = 1.0f / wa_other_sum(lr);
   const bool in = row < w.len;
-  wa_store<D>(out, acc, 1.0f / l, half, in);
+  wa_store<D>(out, acc, lr, half, in, a.low ? a.low + (out - a.out) : nullptr);
   if (in) {
     if (half == 0) a.lse[((int64_t)w.b * a.H + w.head) * a.N + row] = m + __builtin_amdgcn_logf(l);
   } else if (row < a.N) {
@@ -511,11 +543,14 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
   float delta = 0.0f;
   {
     const __bf16* orow = a.o.p + w.b * a.o.sB + w.head * a.o.sH + at * a.o.sN;
+    const __bf16* lrow = a.low + (((int64_t)w.b * a.N + at) * a.H + w.head) * D;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const wa_bf8 of = *(const wa_bf8*)(orow + kk * 16 + half * 8);
+      const wa_bf8 lf = *(const wa_bf8*)(lrow + kk * 16 + half * 8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = fmaf((float)of[j], (float)gf[kk][j], delta);
+      for (int j = 0; j < 8; ++j)
+        delta = fmaf((float)of[j] + (float)lf[j], (float)gf[kk][j], delta);
     }
     delta = wa_other_sum(delta);
   }
@@ -627,7 +662,7 @@ __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int h
 // the other reads) and sums dK and dV over all rows for its half of D.  With
 // full sums in one wave, and K and V in registers as well, D = 128 leaves one
 // wave a SIMD: 738 us where pairs take 461 (8192 rows, 32 over 8 heads, window
-// 1024; 360 with what came later, the rows behind the window included).  PARTS 1: a wave takes all rows and all of D.
+// 1024; 350 with what came later, the rows behind the window included).  PARTS 1: a wave takes all rows and all of D.
 
 template <int D, int PARTS>
 __global__ void __launch_bounds__(PARTS * WA_BLOCK, PARTS == 1 ? 3 : 2)
@@ -941,9 +976,9 @@ static void wa_sum(hipStream_t s, const WaArgs& a, int64_t sums) {
                        dim3(1024), 0, s, a, per, (int)from);
 }
 
-// st: strides (B, H, N) of q, k, v, o, go; o is written as [B, N, H, D]
+// st: strides (B, H, N) of q, k, v, o, go; o and low are written as [B, N, H, D]
 extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void* v,
-                         void* o, float* lse, const int32_t* lengths,
+                         void* o, void* low, float* lse, const int32_t* lengths,
                          const int64_t* st, int64_t B, int64_t H, int64_t KV,
                          int64_t N, int64_t D, int64_t window, int64_t sinks,
                          float scale) {
@@ -951,7 +986,7 @@ extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void*
   WaArgs a{};
   if (int e = wa_fill(a, st, B, H, KV, N, window, sinks, scale, lengths)) return e;
   a.q.p = (const __bf16*)q; a.k.p = (const __bf16*)k; a.v.p = (const __bf16*)v;
-  a.out = (__bf16*)o; a.lse = lse;
+  a.out = (__bf16*)o; a.low = (__bf16*)low; a.lse = lse;
   const int gw = wa_heads_a_block(H / KV);
   const int64_t grid = wa_row_grid(B, H, N, gw);
   if (grid >= WA_MOST / WA_BLOCK || (D != 64 && D != 128)) return 9003;
@@ -962,8 +997,8 @@ extern "C" int ps_wa_fwd(void* stream, const void* q, const void* k, const void*
 }
 
 extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void* v,
-                         const void* o, const void* go, float* lse, float* delta,
-                         void* dq, void* dk, void* dv, float* part,
+                         const void* o, const void* low, const void* go, float* lse,
+                         float* delta, void* dq, void* dk, void* dv, float* part,
                          const int32_t* lengths, const int64_t* st, int64_t B,
                          int64_t H, int64_t KV, int64_t N, int64_t D,
                          int64_t window, int64_t sinks, float scale) {
@@ -971,7 +1006,7 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
   WaArgs a{};
   if (int e = wa_fill(a, st, B, H, KV, N, window, sinks, scale, lengths)) return e;
   a.q.p = (const __bf16*)q; a.k.p = (const __bf16*)k; a.v.p = (const __bf16*)v;
-  a.o.p = (const __bf16*)o; a.go.p = (const __bf16*)go;
+  a.o.p = (const __bf16*)o; a.go.p = (const __bf16*)go; a.low = (__bf16*)low;
   a.lse = lse; a.delta = delta; a.part = part;
   a.dq = (__bf16*)dq; a.dk = (__bf16*)dk; a.dv = (__bf16*)dv;
   const int gw = wa_heads_a_block(H / KV);

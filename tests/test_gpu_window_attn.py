@@ -264,3 +264,51 @@ def test_more_first_tokens_than_a_launch_holds():
         for name, a, b, t in zip(("o", "dq", "dk", "dv"), got, want, tol):
             err = (a[:, h:h + 1].cpu().double() - b).abs()
             assert (err <= t + 1e-30).all(), (h, name, err.max())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks,lengths", [
+    (2, 0, None), (5, 1, None), (40, 0, [150, 61]),
+])
+def test_gradients_of_values_with_a_common_part(D, window, sinks, lengths):
+    """dS = P * (dP - rowsum(dO * O)): a part that all values share cancels.
+    With O rounded to bf16 in that sum its error would not: what the rounding
+    left out is kept, itself rounded, so the sum is off by E * E of its
+    magnitude and the fp32 part S.  O's weights P' are rounded for their product
+    and divided by their own sum: |P' - P| <= 2 E P, and as both add up to 1
+    the sum is off by |sum_j (P' - P)(dP - delta)| <= 2 E sum_j P |dP - delta|,
+    whatever the values share.  The other terms are as in _bounds."""
+    B, H, N = 2, 2, 150
+    q, k, v, go = _make(B, H, 1, N, D, 21)
+    v = (v.float() + 6.0).bfloat16()
+    lens = None if lengths is None else torch.tensor(lengths,
+                                                     dtype=torch.int32)
+    scale = D ** -0.5
+    want = by_hand(q, k, v, go, window, sinks, lens, scale)
+    x = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    o = fused_window_sdpa(*x, window, sinks,
+                          None if lens is None else lens.to(DEV))
+    dq, dk, _ = torch.autograd.grad(o, x, go.to(DEV))
+    tq, tk = E * want[1].abs(), E * want[2].abs()
+    for b in range(B):
+        n = N if lens is None else int(lens[b])
+        i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+        vis = (j <= i) & ((i - j < window) | (j < sinks))
+        K, V = k[b, 0, :n].double(), v[b, 0, :n].double()
+        for h in range(H):
+            Q, R = q[b, h, :n].double(), go[b, h, :n].double()
+            P = torch.softmax((Q @ K.t() * scale).masked_fill(
+                ~vis, -torch.inf), 1)
+            eP = P * S * (1 + (Q.abs() @ K.t().abs() * scale))
+            # P's own fp32 error moves O and with it the sum
+            O = P @ V
+            dd = R @ V.t() - (R * O).sum(1, keepdim=True)
+            edd = (E * E + S) * (R * O).abs().sum(1, keepdim=True) \
+                + S * (R.abs() @ V.t().abs()) \
+                + 2 * E * (P * dd).abs().sum(1, keepdim=True)
+            eS = (E * (P * dd).abs() + eP * dd.abs() + P * edd) * scale
+            tq[b, h, :n] += eS @ K.abs()
+            tk[b, 0, :n] += eS.t() @ Q.abs()
+    for name, a, w, t in (("dq", dq, want[1], tq), ("dk", dk, want[2], tk)):
+        err = (a.cpu().double() - w).abs()
+        assert (err <= t + 1e-30).all(), (name, err.max(), (err / t).max())
