@@ -178,6 +178,8 @@ def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):
     GPU, bf16, D 64 or 128: MFMA kernels forward and backward
     (ops/csrc/window_attn_kernels.hip), reading any strides with unit d stride
     and 16-byte rows.  Anything else: plain torch with the whole score matrix.
+    Where a gradient will be asked for, a second tensor of the output's size is
+    kept for it.
     Values inside the lengths must be finite: a product with a weight of zero
     lets a NaN or infinity reach rows that do not see it.
     """
