@@ -187,6 +187,7 @@ class PS(torch.optim.Optimizer):
         sd = {
             "step_count": self._step_count,
             "bucket_apply_count": dict(self._bucket_apply_count),
+            "bucket_starts": [b.start for b in flat.buckets],
             "names": list(self.names),
             "offsets": [(n, o, sz) for n, p, o, sz in flat.entries],
             "master": flat.master.detach().cpu().clone(),
@@ -202,15 +203,41 @@ class PS(torch.optim.Optimizer):
     def load_state_dict(self, sd):
         flat = self.flat
         assert sd["names"] == self.names, "parameter set mismatch"
+        counts = self._counts_from(sd)  # refuses before anything changes
         self._step_count = sd["step_count"]
-        self._bucket_apply_count = {int(k): v for k, v in
-                                    sd["bucket_apply_count"].items()}
+        self._bucket_apply_count = counts
         flat.master.copy_(sd["master"].to(flat.master.device))
         flat.sync_param_from_master()
         for k, t in self._state_tensors().items():
             t.copy_(sd[k].to(t.device))
         for g, gs in zip(self.param_groups, sd["param_groups"]):
             g.update(gs)
+
+    def _counts_from(self, sd):
+        """The checkpoint's update counts for the buckets of this optimizer,
+        which may be cut at other places."""
+        old = {int(k): v for k, v in sd["bucket_apply_count"].items()}
+        starts = sd.get("bucket_starts")
+        if starts is None:  # written without its buckets' places
+            if len(set(old.values())) <= 1:
+                c = next(iter(old.values()), 0)
+                return {b.idx: c for b in self.flat.buckets if c}
+            if len(old) == len(self.flat.buckets):
+                return old
+            raise ValueError("checkpoint's buckets differ in their number of "
+                             "updates and do not tell where they lie")
+        ends = [*starts[1:], self.flat.total]
+        counts = {}
+        for b in self.flat.buckets:
+            c = {old.get(i, 0) for i, (s, e) in enumerate(zip(starts, ends))
+                 if s < b.end and b.start < e}
+            if len(c) != 1:
+                raise ValueError(
+                    f"elements {b.start} to {b.end} are one bucket here, in "
+                    f"the checkpoint they had {sorted(c)} updates")
+            if c != {0}:
+                counts[b.idx] = c.pop()
+        return counts
 
     def _state_tensors(self):
         return {}

@@ -1,0 +1,65 @@
+"""Checkpoints of the optimizers: resume in other buckets, refusals."""
+
+import pytest
+import torch
+
+from pytorch_ps_mpi_amd import SGD, Adam, AdamW, models
+from test_adamw import _flat, _train
+
+
+@pytest.mark.parametrize("cls,kw", [
+    (AdamW, dict(state_bits=8, seed=5)), (AdamW, dict(state_bits=32)),
+    (Adam, {}), (SGD, dict(momentum=0.9, dampening=0.5))])
+@pytest.mark.parametrize("placed", [True, False])
+def test_checkpoint_resumes_in_other_buckets(cls, kw, placed):
+    """The number of a step (bias corrections, rounding bits, the first
+    momentum) goes with the elements, wherever buckets are cut; checkpoints
+    that do not hold the cuts included."""
+    threads = torch.get_num_threads()
+    torch.set_num_threads(1)  # several split the elementwise loops anew
+
+    def made(mb):
+        torch.manual_seed(0)
+        m = models.build_model("mlp")
+        return m, cls(m.named_parameters(), lr=1e-3, bucket_mb=mb, **kw)
+
+    for first, then in ((50, 0.0001), (0.0001, 50), (0.0001, 0.0001)):
+        m1, o1 = made(first)
+        _train(m1, o1, steps=3)
+        sd = o1.state_dict()
+        if not placed:
+            del sd["bucket_starts"]
+        m2, o2 = made(then)
+        o2.load_state_dict(sd)
+        _train(m1, o1, steps=2, seed=4)
+        _train(m2, o2, steps=2, seed=4)
+        assert set(o2._bucket_apply_count) == set(range(len(o2.flat.buckets)))
+        assert torch.equal(_flat(m1), _flat(m2))
+    torch.set_num_threads(threads)
+
+
+def test_checkpoint_of_uneven_buckets():
+    """Counts that differ stay with their elements, and are refused where one
+    bucket would need two of them, before anything has changed."""
+    def made(mb):
+        torch.manual_seed(0)
+        m = models.build_model("mlp")
+        return m, AdamW(m.named_parameters(), lr=1e-3, bucket_mb=mb)
+
+    m1, o1 = made(0.0001)
+    _train(m1, o1, steps=3)
+    o1._bucket_apply_count[0] = 2
+    sd = o1.state_dict()
+    m2, o2 = made(0.0001)
+    o2.load_state_dict(sd)
+    assert o2._bucket_apply_count == o1._bucket_apply_count
+    for take in (sd, {k: v for k, v in sd.items() if k != "bucket_starts"}):
+        m3, o3 = made(50)
+        before = _flat(m3)
+        with pytest.raises(ValueError, match="updates"):
+            o3.load_state_dict(take)
+        assert torch.equal(_flat(m3), before) and o3._step_count == 0 \
+            and not o3._bucket_apply_count
+    fresh = made(50)[1].state_dict()
+    o2.load_state_dict(fresh)
+    assert not o2._bucket_apply_count
