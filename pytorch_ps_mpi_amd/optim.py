@@ -391,5 +391,6 @@ class AdamW(PS):
             raise ValueError(
                 f"checkpoint holds {sd.get('state_bits')}-bit AdamW states, "
                 f"this optimizer has {self.state_bits}-bit ones")
-        self.seed = sd["seed"]
-        super().load_state_dict(sd)
+        seed = sd["seed"]
+        super().load_state_dict(sd)  # may refuse
+        self.seed = seed

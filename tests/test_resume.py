@@ -63,3 +63,21 @@ def test_checkpoint_of_uneven_buckets():
     fresh = made(50)[1].state_dict()
     o2.load_state_dict(fresh)
     assert not o2._bucket_apply_count
+
+
+def test_refused_checkpoint_leaves_the_seed():
+    """The seed chooses the rounding bits: a checkpoint that is refused, for
+    whatever reason, must not change it."""
+    o1 = AdamW(models.build_model("mlp").named_parameters(), seed=5,
+               state_bits=8)
+    sd = o1.state_dict()
+    m = models.build_model("mlp")
+    o2 = AdamW(m.named_parameters(), seed=9, state_bits=8)
+    before = _flat(m)
+    for bad in (dict(names=["another"]), dict(state_bits=32),
+                dict(bucket_apply_count={0: 1}, bucket_starts=[0, 256])):
+        with pytest.raises((AssertionError, ValueError)):
+            o2.load_state_dict({**sd, **bad})
+        assert o2.seed == 9 and torch.equal(_flat(m), before)
+    o2.load_state_dict(sd)
+    assert o2.seed == 5
