@@ -42,6 +42,7 @@ class CausalBlock(nn.Module):
         self.fc1 = FusedLinear(dim, 4 * dim)
         self.fc2 = FusedLinear(4 * dim, dim)
         self.heads = heads
+        self.g1 = self.g2 = None
         if layer_scale is not None:
             self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
             self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
@@ -70,9 +71,13 @@ class CausalBlock(nn.Module):
         return self.fc2(F.gelu(self.fc1(h)))
 
     def forward(self, x, pos=None):
-        x = x + self.attend(self.n1(x), pos)
-        x = x + self.mlp(self.n2(x))
-        return x
+        u = self.attend(self.n1(x), pos)
+        if self.g1 is None:
+            x = x + u
+            return x + self.mlp(self.n2(x))
+        x, h = fused_gated_residual(x, u, self.n2.weight, self.n2.bias,
+                                    gate=self.g1, eps=self.n2.eps)
+        return x + self.g2 * self.mlp(h)
 
     def joined(self, x, h, after, pos=None):
         """x: residual stream, h: its norm n1.  Returns the stream behind this

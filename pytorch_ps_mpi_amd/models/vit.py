@@ -28,6 +28,7 @@ class Block(nn.Module):
         h = int(dim * mlp_ratio)
         self.fc1 = FusedLinear(dim, h)
         self.fc2 = FusedLinear(h, dim)
+        self.g1 = self.g2 = None
         if layer_scale is not None:
             self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
             self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
@@ -48,9 +49,13 @@ class Block(nn.Module):
         return self.fc2(F.gelu(self.fc1(h)))
 
     def forward(self, x, pos=None):
-        x = x + self.attend(self.n1(x), pos)
-        x = x + self.mlp(self.n2(x))
-        return x
+        u = self.attend(self.n1(x), pos)
+        if self.g1 is None:
+            x = x + u
+            return x + self.mlp(self.n2(x))
+        x, h = fused_gated_residual(x, u, self.n2.weight, self.n2.bias,
+                                    gate=self.g1, eps=self.n2.eps)
+        return x + self.g2 * self.mlp(h)
 
     def joined(self, x, h, after, pos=None):
         x, h = fused_gated_residual(x, self.attend(h, pos), self.n2.weight,

@@ -1,0 +1,41 @@
+"""Blocks with gates on their branches (layer_scale), alone and in a model."""
+
+import pytest
+import torch
+
+from pytorch_ps_mpi_amd.models.gpt2 import GPT2, CausalBlock
+from pytorch_ps_mpi_amd.models.vit import Block, ViT
+
+
+def _block(cls):
+    torch.manual_seed(0)
+    b = cls(64, 2, layer_scale=0.5)
+    with torch.no_grad():  # gates that differ by channel and branch
+        b.g1.copy_(torch.linspace(-1, 1, 64))
+        b.g2.copy_(torch.linspace(2, 0.1, 64))
+    return b
+
+
+@pytest.mark.parametrize("cls", [CausalBlock, Block])
+def test_block_alone_has_its_gates(cls):
+    """As in a model: x + g1 * attention, then + g2 * mlp."""
+    b = _block(cls)
+    x = torch.randn(2, 9, 64, requires_grad=True)
+    y = x + b.g1 * b.attend(b.n1(x))
+    want = y + b.g2 * b.mlp(b.n2(y))
+    got = b(x)
+    # values of up to 10, sums of 256 products: 10 * sqrt(256) * 2^-24 = 1e-5
+    assert torch.allclose(got, want, atol=1e-5)
+    leaves = [x, *b.parameters()]
+    go = torch.randn_like(got)
+    for a, c in zip(torch.autograd.grad(got, leaves, go),
+                    torch.autograd.grad(want, leaves, go)):
+        # as much again in each of some ten steps back
+        assert torch.allclose(a, c, atol=1e-4)
+    with torch.no_grad():
+        b.g1.zero_()
+        b.g2.zero_()
+    assert torch.equal(b(x), x)
+    h = torch.nn.LayerNorm(64)
+    s, n = b.joined(x, b.n1(x), h)
+    assert torch.equal(s, x) and torch.allclose(n, h(x), atol=1e-5)
