@@ -23,7 +23,9 @@ class CausalBlock(nn.Module):
         query heads; rotary : AxialRotary that turns q and k.  Any of them
         takes the windowed kernels, none the full causal ones.
     layer_scale : start value of a gate for each channel of both branches;
-        the norms then ride with gate and residual in one pass (``joined``).
+        the norms then ride with gate and residual in one pass (``joined``):
+        a model calls its blocks, but of its norm modules only the first;
+        the others lend their weights, and hooks on them do not run.
     """
 
     def __init__(self, dim, heads, window=None, sinks=0, kv_heads=None,
@@ -70,7 +72,10 @@ class CausalBlock(nn.Module):
     def mlp(self, h):
         return self.fc2(F.gelu(self.fc1(h)))
 
-    def forward(self, x, pos=None):
+    def forward(self, x, pos=None, h=None, after=None):
+        """x -> x behind this block; with h and ``after``: see ``joined``."""
+        if after is not None:
+            return self.joined(x, h, after, pos)
         u = self.attend(self.n1(x), pos)
         if self.g1 is None:
             x = x + u
@@ -136,7 +141,7 @@ class GPT2(nn.Module):
             norms = [blk.n1 for blk in self.blocks] + [self.norm]
             h = norms[0](x)
             for blk, after in zip(self.blocks, norms[1:]):
-                x, h = blk.joined(x, h, after, pos)
+                x, h = blk(x, pos, h, after)
             x = h
         # tied output head
         return x @ self.wte.weight.t()

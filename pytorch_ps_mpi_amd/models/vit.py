@@ -48,7 +48,10 @@ class Block(nn.Module):
     def mlp(self, h):
         return self.fc2(F.gelu(self.fc1(h)))
 
-    def forward(self, x, pos=None):
+    def forward(self, x, pos=None, h=None, after=None):
+        """x -> x behind this block; with h and ``after``: see ``joined``."""
+        if after is not None:
+            return self.joined(x, h, after, pos)
         u = self.attend(self.n1(x), pos)
         if self.g1 is None:
             x = x + u
@@ -119,7 +122,7 @@ class ViT(nn.Module):
         norms = [blk.n1 for blk in self.blocks] + [self.norm]
         h = norms[0](x)
         for blk, after in zip(self.blocks, norms[1:]):
-            x, h = blk.joined(x, h, after, pos)
+            x, h = blk(x, pos, h, after)
         return self.head(h[:, 0])
 
 

@@ -39,3 +39,33 @@ def test_block_alone_has_its_gates(cls):
     h = torch.nn.LayerNorm(64)
     s, n = b.joined(x, b.n1(x), h)
     assert torch.equal(s, x) and torch.allclose(n, h(x), atol=1e-5)
+
+
+def _models():
+    torch.manual_seed(0)
+    yield (GPT2(vocab=31, ctx=16, dim=64, depth=3, heads=2, layer_scale=0.5),
+           torch.randint(0, 31, (2, 9)))
+    yield (ViT(img=16, patch=8, dim=64, depth=3, heads=2, num_classes=5,
+               layer_scale=0.5), torch.randn(2, 3, 16, 16))
+
+
+def test_models_call_their_gated_blocks():
+    """Hooks of a block and wrappers of its forward see every step, and what
+    they return counts."""
+    for m, x in _models():
+        want, seen = m(x), []
+        for i, b in enumerate(m.blocks):
+            b.register_forward_hook(
+                lambda mod, args, out, i=i: seen.append((i, len(out))))
+        assert torch.equal(m(x), want)
+        assert seen == [(0, 2), (1, 2), (2, 2)]
+        inner = m.blocks[1].forward
+        m.blocks[1].forward = lambda *a, **k: torch.utils.checkpoint \
+            .checkpoint(inner, *a, use_reentrant=False, **k)
+        got = m(x)
+        assert torch.equal(got, want)
+        got.sum().backward()
+        assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+        m.blocks[2].register_forward_hook(
+            lambda mod, args, out: (out[0], out[1] * 0))
+        assert torch.equal(m(x)[0], m(x)[1])
