@@ -161,7 +161,11 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
                                   top))
     total = e.sum(3, keepdim=True)
     p = e / torch.where(total == 0, torch.ones_like(total), total)
-    return (p @ vf).to(q.dtype)
+    o = p @ vf
+    if lengths is not None:
+        # nor is a gradient that comes from there
+        o = o.masked_fill(past, 0)
+    return o.to(q.dtype)
 
 
 def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):

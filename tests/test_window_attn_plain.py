@@ -1,0 +1,46 @@
+"""The path of windowed attention without a kernel: CPU, and other types and
+head sizes on the GPU.  It keeps the kernels' promises."""
+
+import pytest
+import torch
+
+from pytorch_ps_mpi_amd.ops.attn import fused_window_sdpa
+
+GPU = pytest.param("cuda:0", marks=pytest.mark.gpu)
+
+
+def _run(q, k, v, go, *args):
+    x = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    o = fused_window_sdpa(*x, *args)
+    return [o.detach(), *torch.autograd.grad(o, x, go)]
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16,
+                                   torch.bfloat16])
+@pytest.mark.parametrize("bad", [torch.nan, torch.inf, -torch.inf])
+def test_what_stands_behind_a_length_goes_nowhere(device, dtype, bad):
+    """In q, k, v and in the output's gradient, by itself and all at once."""
+    g = torch.Generator().manual_seed(0)
+    B, N, D = 5, 9, 24  # a head size without a kernel
+    lengths = [9, 4, 0, 1, 99]
+    t = [torch.randn(B, h, N, D, generator=g).to(device, dtype)
+         for h in (4, 2, 2, 4)]
+    lens = torch.tensor(lengths, dtype=torch.int32, device=device)
+    clean = []
+    for x in t:
+        c = x.clone()
+        for b, n in enumerate(lengths):
+            c[b, :, n:] = 0
+        clean.append(c)
+    want = _run(*clean, 3, 1, lens)
+    for which in ((0,), (1,), (2,), (3,), (0, 1, 2, 3)):
+        dirty = [c.clone() for c in clean]
+        for i in which:
+            for b, n in enumerate(lengths):
+                dirty[i][b, :, n:] = bad
+        got = _run(*dirty, 3, 1, lens)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y), which
+            for b, n in enumerate(lengths):
+                assert (x[b, :, n:] == 0).all()
