@@ -156,7 +156,8 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
         q, kf, vf = (x.masked_fill(past, 0) for x in (q, kf, vf))
     z = (q.to(t) @ kf.transpose(2, 3).contiguous()) * scale
     z = z.masked_fill(~vis[:, None], -math.inf)
-    top = z.detach().amax(3, keepdim=True)
+    # a row of no keys has no maximum
+    top = z.detach().amax(3, keepdim=True) if N else z.detach().sum(3, True)
     e = torch.exp(z - torch.where(top == -math.inf, torch.zeros_like(top),
                                   top))
     total = e.sum(3, keepdim=True)
@@ -193,6 +194,8 @@ def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):
     if k.shape[0] != B or k.shape[2] != N or k.shape[3] != D:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ "
                          "in B, N or D")
+    if D < 1:
+        raise ValueError("heads must have at least one element")
     if k.shape[1] < 1 or H % k.shape[1]:
         raise ValueError(f"{H} query heads do not divide over {k.shape[1]} "
                          "key heads")

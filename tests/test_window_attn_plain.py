@@ -44,3 +44,25 @@ def test_what_stands_behind_a_length_goes_nowhere(device, dtype, bad):
             assert torch.equal(x, y), which
             for b, n in enumerate(lengths):
                 assert (x[b, :, n:] == 0).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,KV,N", [(2, 4, 2, 0), (0, 4, 2, 5), (0, 4, 2, 0),
+                                      (2, 0, 2, 5)])
+@pytest.mark.parametrize("padded", [False, True])
+def test_empty(device, dtype, B, H, KV, N, padded):
+    """No rows, no sequences or no query heads: an empty result with a graph
+    behind it, zeros for keys that nothing looks at."""
+    mk = lambda h: torch.randn(B, h, N, 64, device=device, dtype=dtype)  # noqa: E731
+    lens = torch.ones(B, dtype=torch.int32, device=device) if padded else None
+    o, dq, dk, dv = _run(mk(H), mk(KV), mk(KV), mk(H), 3, 1, lens)
+    assert o.shape == dq.shape == (B, H, N, 64)
+    assert dk.shape == dv.shape == (B, KV, N, 64)
+    assert o.dtype == dtype and not dk.any() and not dv.any()
+
+
+def test_heads_without_elements_are_refused():
+    t = torch.empty(2, 2, 3, 0)
+    with pytest.raises(ValueError, match="one element"):
+        fused_window_sdpa(t, t, t, 3)
