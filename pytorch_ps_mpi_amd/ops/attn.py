@@ -166,7 +166,7 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
     if lengths is not None:
         # nor is a gradient that comes from there
         o = o.masked_fill(past, 0)
-    return o.to(q.dtype)
+    return o.to(q.dtype).transpose(1, 2).contiguous().transpose(1, 2)
 
 
 def fused_window_sdpa(q, k, v, window, sinks=0, lengths=None, scale=None):

@@ -66,3 +66,15 @@ def test_heads_without_elements_are_refused():
     t = torch.empty(2, 2, 3, 0)
     with pytest.raises(ValueError, match="one element"):
         fused_window_sdpa(t, t, t, 3)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_heads_are_stored_behind_the_rows(device, dtype):
+    """The documented layout, whichever path computes: a view of it is what a
+    projection of all heads reads."""
+    q, k = (torch.randn(2, h, 7, 64, device=device, dtype=dtype)
+            for h in (4, 2))
+    o = fused_window_sdpa(q, k, k, 3)
+    assert o.transpose(1, 2).is_contiguous()
+    assert o.transpose(1, 2).view(2, 7, 4 * 64).data_ptr() == o.data_ptr()
