@@ -135,6 +135,9 @@ class State8:
 
     def span(self, start, end):
         """State8 of elements [start, end), sharing storage."""
+        if not 0 <= start <= end <= self.codes.numel():
+            raise ValueError(f"span [{start}, {end}) of a state of "
+                             f"{self.codes.numel()} elements")
         if start % ACHUNK:
             raise ValueError(f"a span starts at a multiple of {ACHUNK}")
         if end % ACHUNK and end != self.codes.numel():
