@@ -234,7 +234,8 @@ def fused_adamw(p, m1, m2, g, p_out=None, *, lr, beta1=0.9, beta2=0.999,
         with the probability that keeps its mean, from bits that depend on
         (offset + element index, seed, step) alone: a buffer updated in parts
         (``offset`` = where the part starts) rounds as it would in one.
-        An infinity or NaN makes the values of its 256 elements read as NaN.
+        An infinity or NaN in one of the states makes that state's values of
+        its 256 elements read as NaN.
     step : counts from 1; it enters as a number, so a captured graph repeats
         the step that it was captured with.
     """

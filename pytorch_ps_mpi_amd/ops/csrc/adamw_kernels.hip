@@ -16,8 +16,8 @@
 // upper one with the probability that keeps its mean.  The 16 random bits come
 // from a 32-bit mix of (element index, seed, step): every rank and every
 // bucketing rounds alike.  A second moment that is not zero keeps at least the
-// lowest code, so that no denominator collapses to eps.  A chunk that holds an
-// infinity or NaN gets the maximum NaN: all its values read as NaN.
+// lowest code, so that no denominator collapses to eps.  A state's chunk that
+// holds an infinity or NaN gets the maximum NaN: all its values read as NaN.
 //
 // Bound by HBM: 30 bytes an element with fp32 states and a bf16 copy, 18 with
 // 8-bit states.  124 M elements: 679 us (5.5 TB/s) and 482 us (4.6 TB/s).
@@ -216,18 +216,19 @@ __device__ __forceinline__ void aw_chunk(const AwArgs& a, int64_t c, int lane) {
   }
   if (S8) {
     float am = 0, av = 0;
-    bool bad = false;
+    bool mbad = false, vbad = false;  // one may overflow without the other
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!VEC && i0 + j >= a.n) m[j] = v[j] = 0.0f;
       am = fmaxf(am, fabsf(m[j]));
       av = fmaxf(av, v[j]);
-      // m and v come from the same g: one sum shows an infinity or NaN
-      bad |= !(fabsf(m[j]) + v[j] < INFINITY);
+      mbad |= !(fabsf(m[j]) < INFINITY);
+      vbad |= !(v[j] < INFINITY);
     }
     am = aw_wave_max(am);
     av = aw_wave_max(av);
-    if (__any(bad)) am = av = NAN;
+    if (__any(mbad)) am = NAN;
+    if (__any(vbad)) av = NAN;
     float mx = am, vx = av, ml, mi, vl, vi;
     aw_lift(mx, ml, mi);
     aw_lift(vx, vl, vi);
