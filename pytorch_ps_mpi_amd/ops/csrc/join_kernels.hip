@@ -445,6 +445,7 @@ struct JoinSums {
   void* out[5];     // by slot
   const float* part;
   int slots, slot_g, groups, nb, D;
+  int from;         // first of the sums that this launch takes
 };
 
 // out[slot][d] = sum over blocks of part[block][slot][d]; the gate's slot one
@@ -456,16 +457,16 @@ __global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
   const int d = blockIdx.x * 32 + col;
   // y: first the slots summed over all blocks, then the gate's groups
   const bool each = a.slot_g >= 0 && a.groups > 1;
-  const int whole = a.slots - (each ? 1 : 0);
+  const int whole = a.slots - (each ? 1 : 0), y = a.from + (int)blockIdx.y;
   int slot, first, count, g = 0;
-  if ((int)blockIdx.y < whole) {
-    slot = blockIdx.y;
+  if (y < whole) {
+    slot = y;
     if (each && slot >= a.slot_g) ++slot;
     first = 0;
     count = a.groups * a.nb;
   } else {
     slot = a.slot_g;
-    g = blockIdx.y - whole;
+    g = y - whole;
     first = g * a.nb;
     count = a.nb;
   }
@@ -559,8 +560,8 @@ extern "C" int64_t ps_join_blocks(int64_t groups, int64_t rows, int64_t D, int p
 }
 
 static int jn_check(const JoinArgs& a, int64_t groups) {
-  if (a.D < 1 || a.D > JN_MAXD || groups > 65530 || groups * a.nb > 0x7fffffff)
-    return 9003;
+  // a launch holds fewer than 2^32 threads, 512 a block at most
+  if (a.D < 1 || a.D > JN_MAXD || groups * a.nb >= 1 << 23) return 9003;
   return 0;
 }
 
@@ -615,8 +616,14 @@ extern "C" int ps_join_bwd(void* stream, void* const* t, float* const* stats,
   q.part = part; q.slots = a.slots; q.slot_g = a.slot_g;
   q.groups = (int)groups; q.nb = a.nb; q.D = (int)D;
   const int gy = a.slots + (a.slot_g >= 0 && groups > 1 ? (int)groups - 1 : 0);
-  const dim3 sg((unsigned)((D + 31) / 32), (unsigned)gy);
-  if (bf16) hipLaunchKernelGGL((k_join_sum<__hip_bfloat16>), sg, dim3(1024), 0, s, q);
-  else hipLaunchKernelGGL((k_join_sum<float>), sg, dim3(1024), 0, s, q);
+  // a grid has at most 65535 rows and here, with up to 256 columns of 1024
+  // threads, fewer than 2^32 threads: more samples' gates take several launches
+  constexpr int MOST = 1 << 13;
+  for (; q.from < gy; q.from += MOST) {
+    const dim3 sg((unsigned)((D + 31) / 32),
+                  (unsigned)(gy - q.from < MOST ? gy - q.from : MOST));
+    if (bf16) hipLaunchKernelGGL((k_join_sum<__hip_bfloat16>), sg, dim3(1024), 0, s, q);
+    else hipLaunchKernelGGL((k_join_sum<float>), sg, dim3(1024), 0, s, q);
+  }
   return (int)hipGetLastError();
 }

@@ -100,7 +100,8 @@ def fused_gated_residual(x, u, weight, bias=None, *, gate=None,
     shape.  The norm is taken of y before its rounding.
 
     GPU: HIP kernels (ops/csrc/join_kernels.hip) for bf16 and fp32, D up to
-    8192; other types or sizes raise.  CPU: plain torch, the oracle.
+    8192, gates of fewer than 2**23 samples; other types or sizes raise.  CPU:
+    plain torch, the oracle.
     """
     if kind not in ("layer", "rms"):
         raise ValueError(f"kind must be 'layer' or 'rms', got {kind!r}")
