@@ -626,11 +626,11 @@ __global__ void __launch_bounds__(WA_BLOCK, 2) k_wa_dq(const WaArgs a, int gw) {
 // ---------------------------------------------------------------------------
 // backward: dK and dV
 // ---------------------------------------------------------------------------
-// The first tile of rows that see none of keys k0..k0+127 by the window.
+// The first tile of rows that see none of keys k0..k0+127 by the window.  Where
+// no blocks take the rest (slots = 0) there is none: no first tokens, or a
+// window that covers the sequence.
 __device__ __forceinline__ int wa_behind(const WaArgs& a, int k0, int len) {
   const int64_t end = (int64_t)k0 + WA_KB - 1 + a.window;
-  // where no blocks take the rest the last tile is the sequence's
-  if (a.slots == 0 && k0 < a.sinks) return (len + WA_T - 1) / WA_T;
   return (int)((min(end, (int64_t)len) + WA_T - 1) / WA_T);
 }
 
