@@ -25,7 +25,7 @@ _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _rotate_plain(x, cos, sin, interleaved):
     P = cos.shape[-1]
-    f = x if x.dtype == torch.float64 else x.float()
+    f = x.float()
     r, rest = f[..., :2 * P], f[..., 2 * P:]
     if interleaved:
         a, b = r[..., 0::2], r[..., 1::2]
