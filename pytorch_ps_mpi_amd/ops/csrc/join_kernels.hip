@@ -490,10 +490,10 @@ __global__ void __launch_bounds__(1024) k_join_sum(const JoinSums a) {
 // ---------------------------------------------------------------------------
 
 // Lanes and elements a lane for a row of D.  Eight elements a lane keep the
-// backward kernel with Post, or in fp32, at two waves a SIMD (16 took 256
-// registers and left one); else 16 fit.  A lane's vectors are 16 bytes wide even where
-// that leaves lanes idle: rows of 768 as 64 lanes of 12 elements in vectors of
-// 8 bytes took 155 us backward where 64 lanes of 16 take 92 (49152 rows).
+// backward kernel with Post, or in fp32, at two or three waves a SIMD (16 took
+// 256 registers and left one); else 16 fit, with two, and one wave a row beats
+// two (49152 rows of 768 backward: 116 us, as 128 lanes of 8 167).  A lane's
+// vectors are 16 bytes wide even where that leaves a quarter of the lanes idle.
 struct JnShape {
   int ept, tpr;
 };
@@ -536,8 +536,11 @@ static void jn_pick(hipStream_t s, int grid, const JoinArgs& a) {
   else jn_launch<T, BWD, false, 0>(s, grid, a);
 }
 
-// Blocks of a group: the backward kernel's registers let 2048 waves be on the
-// chip at once; more would only write more parts.  Forward 4096 waves: each
+// Blocks of a group.  Backward 2048 waves: what the registers of most forms let
+// be on the chip at once; more would only write more parts.  Rows of at most 512
+// without Post leave room for 3072 to 5120, which 4096 waves use at 256 elements
+// (196608 rows: 294 us with 2048, 184 with 4096) and not at 512 (98304 rows: 117
+// and 125; with Post 118 and 125).  Forward 4096 waves: each
 // reads the weights once (49152 rows of 768: 62 us with 8192, 58 with 4096).
 // Rows of 256 lanes with Post wait at more barriers and want 8192 (8192 rows of
 // 4096: 59 us with 4096, 55 with 8192; 16384 of 1536: 54 and 48), without Post

@@ -162,8 +162,9 @@ __device__ __forceinline__ void wa_row(const __bf16* row, int half, wa_bf8* f) {
 // A tile on its way from memory to LDS, without registers: each of NW waves
 // moves pieces of 1 KB, lane i to the piece's 16 bytes number i; the swizzle is
 // on the side of memory.  Whole tiles are addressed by a scalar base and a
-// 32-bit offset a lane; in the last one rows past the length take the last
-// one's place: what stands there is never read.
+// 32-bit offset a lane; in the last one rows past the length hold the last row
+// again.  Those are multiplied like others and get the weight zero (a mask; in
+// dK/dV a statistic of infinity), which only finite values let vanish.
 template <int D, int NW>
 struct WaMove {
   static constexpr int G = D / 8, R = 64 / G, CNT = WA_T / R / NW;
@@ -663,7 +664,9 @@ __device__ __forceinline__ void wa_store_part(float* row, const wa_f16* f, int h
 // the other reads) and sums dK and dV over all rows for its half of D.  With
 // full sums in one wave, and K and V in registers as well, D = 128 leaves one
 // wave a SIMD: 738 us where pairs take 461 (8192 rows, 32 over 8 heads, window
-// 1024; 350 with what came later, the rows behind the window included).  PARTS 1: a wave takes all rows and all of D.
+// 1024; 350 with what came later, the rows behind the window included).  PARTS 1:
+// a wave takes all rows and all of D; at three waves a SIMD it keeps 8 of its
+// registers (32 bytes a lane) in scratch.
 
 template <int D, int PARTS>
 __global__ void __launch_bounds__(PARTS * WA_BLOCK, PARTS == 1 ? 3 : 2)
@@ -1027,8 +1030,9 @@ extern "C" int ps_wa_bwd(void* stream, const void* q, const void* k, const void*
   if (D == 64) {
     hipLaunchKernelGGL((k_wa_dq<64>), rows, dim3(WA_BLOCK), 0, s, a, gw);
     // Pairs of waves where blocks do not fill the chip by themselves (16 key
-    // heads of 2048: 66 us against 102), else one wave for both (96 of 1024:
-    // 31 us against 41).
+    // heads of 2048, 256 blocks: 66 us against 102), else one wave for both (96
+    // of 1024, 768 blocks: 31 us against 41).  The border lies between these
+    // two; blocks for rows behind the window count as others.
     if (kgrid < 512)
       hipLaunchKernelGGL((k_wa_dkv<64, 2>), keys, dim3(2 * WA_BLOCK), 0, s, a);
     else
