@@ -21,7 +21,7 @@
 // or NaN gets the maximum NaN: all its values read as NaN.
 //
 // Bound by HBM: 30 bytes an element with fp32 states and a bf16 copy, 18 with
-// 8-bit states.  124 M elements: 679 us (5.5 TB/s) and 482 us (4.6 TB/s).
+// 8-bit states.  124 M elements: 678 us (5.5 TB/s) and 489 us (4.6 TB/s).
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>

@@ -917,7 +917,7 @@ static int wa_slots(int64_t U, int64_t G, int64_t N, int64_t window, int64_t sin
 
 // Blocks that share the rows of 128 keys where there are fewer of those than
 // CUs: one round of blocks, with at least four (head, tile) pairs each.  6 sequences of
-// 777, 8 over 2 heads of 128, window 100: 43 us in 84 blocks, 26 in 252.
+// 777, 8 over 2 heads of 128, window 100: 43 us in 84 blocks, 25 in 252.
 static int wa_splits(int64_t U, int64_t G, int64_t N, int64_t window) {
   const int64_t blocks = U * ((N + WA_KB - 1) / WA_KB);
   const int64_t rows = window + WA_KB < N ? window + WA_KB : N;
