@@ -137,6 +137,27 @@ def fused_sdpa(q, k, v, is_causal=False):
 # sliding window with first tokens that stay visible
 # ---------------------------------------------------------------------------
 
+class _Product(torch.autograd.Function):
+    """a @ b in their own type: autocast would make both passes bf16."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(a, b):
+        with torch.autocast(a.device.type, enabled=False):
+            return a @ b
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs)
+
+    @staticmethod
+    def backward(ctx, g):
+        a, b = ctx.saved_tensors
+        with torch.autocast(a.device.type, enabled=False):
+            return g @ b.transpose(-2, -1), a.transpose(-2, -1) @ g
+
+
 def _window_plain(q, k, v, window, sinks, lengths, scale):
     """The whole score matrix in fp32 (fp64 for fp64): oracle, and the path of
     types and head sizes that have no kernel."""
@@ -154,7 +175,7 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
         # what stands behind a sequence is not looked at, NaN included
         past = (torch.arange(N, device=q.device) >= n[:, 0])[:, None, :, None]
         q, kf, vf = (x.masked_fill(past, 0) for x in (q, kf, vf))
-    z = (q.to(t) @ kf.transpose(2, 3).contiguous()) * scale
+    z = _Product.apply(q.to(t), kf.transpose(2, 3).contiguous()) * scale
     z = z.masked_fill(~vis[:, None], -math.inf)
     # a row of no keys has no maximum
     top = z.detach().amax(3, keepdim=True) if N else z.detach().sum(3, True)
@@ -162,7 +183,7 @@ def _window_plain(q, k, v, window, sinks, lengths, scale):
                                   top))
     total = e.sum(3, keepdim=True)
     p = e / torch.where(total == 0, torch.ones_like(total), total)
-    o = p @ vf
+    o = _Product.apply(p, vf)
     if lengths is not None:
         # nor is a gradient that comes from there
         o = o.masked_fill(past, 0)

@@ -78,3 +78,24 @@ def test_heads_are_stored_behind_the_rows(device, dtype):
     o = fused_window_sdpa(q, k, k, 3)
     assert o.transpose(1, 2).is_contiguous()
     assert o.transpose(1, 2).view(2, 7, 4 * 64).data_ptr() == o.data_ptr()
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("padded", [False, True])
+def test_autocast_leaves_the_sums_in_32_bits(device, dtype, padded):
+    """The path promises scores and sums in 32 bits; autocast would turn its
+    products into bf16 ones, forward and backward."""
+    g = torch.Generator().manual_seed(0)
+    t = [torch.randn(2, h, 9, 24, generator=g).to(device, dtype)
+         for h in (4, 2, 2, 4)]
+    lens = torch.tensor([9, 4], dtype=torch.int32,
+                        device=device) if padded else None
+    want = _run(*t, 3, 1, lens)
+    with torch.autocast(t[0].device.type, dtype=torch.bfloat16):
+        got = _run(*t, 3, 1, lens)
+        x = [v.clone().requires_grad_() for v in t[:3]]
+        o = fused_window_sdpa(*x, 3, 1, lens)
+    later = [o.detach(), *torch.autograd.grad(o, x, t[3])]
+    for a, b, c in zip(want, got, later):
+        assert a.dtype == b.dtype and torch.equal(a, b) and torch.equal(a, c)
