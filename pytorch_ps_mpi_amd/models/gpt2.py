@@ -80,18 +80,20 @@ class CausalBlock(nn.Module):
         if self.g1 is None:
             x = x + u
             return x + self.mlp(self.n2(x))
-        x, h = fused_gated_residual(x, u, self.n2.weight, self.n2.bias,
-                                    gate=self.g1, eps=self.n2.eps)
+        x, h = fused_gated_residual(x, u.to(x.dtype), self.n2.weight,
+                                    self.n2.bias, gate=self.g1,
+                                    eps=self.n2.eps)
         return x + self.g2 * self.mlp(h)
 
     def joined(self, x, h, after, pos=None):
         """x: residual stream, h: its norm n1.  Returns the stream behind this
-        block and its norm by ``after``."""
-        x, h = fused_gated_residual(x, self.attend(h, pos), self.n2.weight,
-                                    self.n2.bias, gate=self.g1,
-                                    eps=self.n2.eps)
-        return fused_gated_residual(x, self.mlp(h), after.weight, after.bias,
-                                    gate=self.g2, eps=after.eps)
+        block and its norm by ``after``.  Branches take the stream's type:
+        under autocast they come back in fewer bits."""
+        x, h = fused_gated_residual(x, self.attend(h, pos).to(x.dtype),
+                                    self.n2.weight, self.n2.bias,
+                                    gate=self.g1, eps=self.n2.eps)
+        return fused_gated_residual(x, self.mlp(h).to(x.dtype), after.weight,
+                                    after.bias, gate=self.g2, eps=after.eps)
 
 
 class GPT2(nn.Module):

@@ -56,16 +56,17 @@ class Block(nn.Module):
         if self.g1 is None:
             x = x + u
             return x + self.mlp(self.n2(x))
-        x, h = fused_gated_residual(x, u, self.n2.weight, self.n2.bias,
-                                    gate=self.g1, eps=self.n2.eps)
+        x, h = fused_gated_residual(x, u.to(x.dtype), self.n2.weight,
+                                    self.n2.bias, gate=self.g1,
+                                    eps=self.n2.eps)
         return x + self.g2 * self.mlp(h)
 
     def joined(self, x, h, after, pos=None):
-        x, h = fused_gated_residual(x, self.attend(h, pos), self.n2.weight,
-                                    self.n2.bias, gate=self.g1,
-                                    eps=self.n2.eps)
-        return fused_gated_residual(x, self.mlp(h), after.weight, after.bias,
-                                    gate=self.g2, eps=after.eps)
+        x, h = fused_gated_residual(x, self.attend(h, pos).to(x.dtype),
+                                    self.n2.weight, self.n2.bias,
+                                    gate=self.g1, eps=self.n2.eps)
+        return fused_gated_residual(x, self.mlp(h).to(x.dtype), after.weight,
+                                    after.bias, gate=self.g2, eps=after.eps)
 
 
 class ViT(nn.Module):

@@ -69,3 +69,34 @@ def test_models_call_their_gated_blocks():
         m.blocks[2].register_forward_hook(
             lambda mod, args, out: (out[0], out[1] * 0))
         assert torch.equal(m(x)[0], m(x)[1])
+
+
+@pytest.mark.parametrize("alone", [False, True])
+def test_gated_blocks_under_autocast(alone):
+    """Branches come back in bf16, the residual stream stays in fp32, as
+    without gates: a model with gates of one is the default one.  Both paths
+    round the same values to bf16; where they lie within fp32 rounding of a
+    border they differ by a step, 2^-7, of one value of many: the norm of the
+    difference stays under that of all."""
+    for make, x in (
+            (lambda **k: GPT2(vocab=31, ctx=16, dim=64, depth=2, heads=2, **k),
+             torch.randint(0, 31, (2, 9))),
+            (lambda **k: ViT(img=16, patch=8, dim=64, depth=2, heads=2,
+                             num_classes=5, **k),
+             torch.randn(2, 3, 16, 16))):
+        torch.manual_seed(0)
+        a, b = make(), make(layer_scale=1.0)
+        b.load_state_dict({**b.state_dict(), **a.state_dict()})
+        if alone:
+            a, b = a.blocks[1], b.blocks[1]
+            x = torch.randn(2, 7, 64)
+        got = []
+        for m in (a, b):
+            with torch.autocast("cpu", dtype=torch.bfloat16):
+                y = m(x)
+            y.float().square().sum().backward()
+            got.append((y.detach().float(), dict(m.named_parameters())))
+        assert (got[0][0] - got[1][0]).norm() <= 2 ** -7 * got[0][0].norm()
+        for n, p in got[0][1].items():
+            g = got[1][1][n].grad
+            assert (p.grad - g).norm() <= 2 ** -5 * p.grad.norm() + 1e-6, n
