@@ -1,0 +1,129 @@
+"""The transformer-step operators as programs call them (@gpu): without a
+graph, recomputed in the backward pass, from several threads and streams, with
+tensors of other ranks."""
+
+import threading
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from pytorch_ps_mpi_amd.models.gpt2 import GPT2
+from pytorch_ps_mpi_amd.models.vit import ViT
+from pytorch_ps_mpi_amd.ops.attn import fused_window_sdpa
+from pytorch_ps_mpi_amd.ops.ln import fused_gated_residual
+from pytorch_ps_mpi_amd.ops.rope import AxialRotary
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _models():
+    for make, x in (
+            (lambda: GPT2(vocab=64, ctx=80, dim=128, depth=2, heads=2,
+                          window=20, sinks=2, kv_heads=1, rotary=True,
+                          layer_scale=0.5), torch.randint(0, 64, (2, 70))),
+            (lambda: ViT(img=32, patch=8, dim=128, depth=2, heads=2,
+                         num_classes=8, rotary=True, layer_scale=0.5),
+             torch.randn(2, 3, 32, 32).bfloat16())):
+        torch.manual_seed(0)
+        yield make().to(DEV, torch.bfloat16), x.to(DEV)
+
+
+def test_without_a_graph():
+    for m, x in _models():
+        want = m(x)
+        with torch.no_grad():
+            assert torch.equal(m(x), want)
+        with torch.inference_mode():
+            got = m(x)
+        assert torch.equal(got, want) and not got.requires_grad
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_blocks_recomputed_in_the_backward_pass(reentrant):
+    for m, x in _models():
+        want = m(x)
+        want.float().square().sum().backward()
+        grads = [p.grad.clone() for p in m.parameters()]
+        m.zero_grad()
+        for b in m.blocks:
+            inner = b.forward
+            b.forward = lambda *a, inner=inner: checkpoint(
+                inner, *a, use_reentrant=reentrant)
+        got = m(x)
+        assert torch.equal(got, want)
+        got.float().square().sum().backward()
+        for p, g in zip(m.parameters(), grads):
+            assert torch.equal(p.grad, g)
+
+
+def test_several_threads_on_streams_of_their_own():
+    """Workspaces belong to a call: four threads at once get what one gets."""
+    g = torch.Generator().manual_seed(0)
+    rot = AxialRotary(64, (20, 12))
+    pos = torch.stack([torch.arange(300), torch.arange(300) // 7]).to(DEV)
+    w = torch.randn(256, generator=g).bfloat16().to(DEV).requires_grad_()
+    inputs = [[torch.randn(2, 300, h, 64, generator=g).bfloat16().to(DEV)
+               for h in (4, 2, 2, 4)] for _ in range(4)]
+
+    def run(t):
+        q, k, v = (x.detach().requires_grad_() for x in t[:3])
+        a, b = rot(q, k, pos)
+        o = fused_window_sdpa(a.transpose(1, 2), b.transpose(1, 2),
+                              v.transpose(1, 2), 50, 3).transpose(1, 2)
+        y, h = fused_gated_residual(t[3].flatten(2), o.flatten(2), w)
+        return [y.detach(), h.detach(),
+                *torch.autograd.grad((y, h), (q, k, v, w), (h, y))]
+
+    want = [run(t) for t in inputs]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    got[i] = run(inputs[i])
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001 (shown by the assertion)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+def test_join_of_other_ranks(gate):
+    g = torch.Generator().manual_seed(1)
+    x, u, gy, gh = (torch.randn(24, 96, generator=g).to(DEV)
+                    for _ in range(4))
+    w = torch.randn(96, generator=g).to(DEV)
+    t = dict(none=None, channel=w * 0.5, token=u * 0.3)[gate]
+
+    def run(*shape):
+        v = [a.reshape(*shape, 96).requires_grad_() for a in (x, u)]
+        gt = t.reshape(*shape, 96) if gate == "token" else t
+        if gt is not None:
+            gt = gt.detach().requires_grad_()
+        y, h = fused_gated_residual(*v, w, gate=gt)
+        leaves = v + ([] if gt is None else [gt])
+        d = torch.autograd.grad((y, h), leaves, (gy.reshape(*shape, 96),
+                                                 gh.reshape(*shape, 96)))
+        return [a.detach().reshape(-1, 96) for a in (y, h, *d)]
+
+    want = run(24)
+    for shape in ((2, 12), (2, 3, 4), (1, 2, 2, 6)):
+        for a, b in zip(run(*shape), want):
+            assert torch.equal(a, b)
+    y, h = fused_gated_residual(x[0], u[0], w)
+    assert torch.equal(torch.stack([y, h]), torch.stack(
+        [a[0] for a in fused_gated_residual(x, u, w)]))
