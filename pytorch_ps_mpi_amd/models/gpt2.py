@@ -6,26 +6,23 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
 from ..ops.attn import fused_sdpa_qkv, fused_window_sdpa
 from ..ops.ce import fused_cross_entropy
 from ..ops.linear import FusedLinear
-from ..ops.ln import FusedLayerNorm, fused_gated_residual
+from ..ops.ln import FusedLayerNorm
 from ..ops.rope import AxialRotary
+from .block import TwoBranches
 
 
-class CausalBlock(nn.Module):
+class CausalBlock(TwoBranches):
     """One transformer block.
 
     window, sinks : attention to the last ``window`` tokens and the first
         ``sinks`` ones; kv_heads : key heads, each shared by heads/kv_heads
         query heads; rotary : AxialRotary that turns q and k.  Any of them
         takes the windowed kernels, none the full causal ones.
-    layer_scale : start value of a gate for each channel of both branches;
-        the norms then ride with gate and residual in one pass (``joined``):
-        a model calls its blocks, but of its norm modules only the first;
-        the others lend their weights, and hooks on them do not run.
+    layer_scale : start value of the gates (models/block.py).
     """
 
     def __init__(self, dim, heads, window=None, sinks=0, kv_heads=None,
@@ -44,10 +41,7 @@ class CausalBlock(nn.Module):
         self.fc1 = FusedLinear(dim, 4 * dim)
         self.fc2 = FusedLinear(4 * dim, dim)
         self.heads = heads
-        self.g1 = self.g2 = None
-        if layer_scale is not None:
-            self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
-            self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
+        self.add_gates(dim, layer_scale)
 
     def attend(self, h, pos=None):
         B, T, D = h.shape
@@ -68,32 +62,6 @@ class CausalBlock(nn.Module):
                                   T if self.window is None else self.window,
                                   self.sinks)
         return self.proj(y.transpose(1, 2).reshape(B, T, D))
-
-    def mlp(self, h):
-        return self.fc2(F.gelu(self.fc1(h)))
-
-    def forward(self, x, pos=None, h=None, after=None):
-        """x -> x behind this block; with h and ``after``: see ``joined``."""
-        if after is not None:
-            return self.joined(x, h, after, pos)
-        u = self.attend(self.n1(x), pos)
-        if self.g1 is None:
-            x = x + u
-            return x + self.mlp(self.n2(x))
-        x, h = fused_gated_residual(x, u.to(x.dtype), self.n2.weight,
-                                    self.n2.bias, gate=self.g1,
-                                    eps=self.n2.eps)
-        return x + self.g2 * self.mlp(h)
-
-    def joined(self, x, h, after, pos=None):
-        """x: residual stream, h: its norm n1.  Returns the stream behind this
-        block and its norm by ``after``.  Branches take the stream's type:
-        under autocast they come back in fewer bits."""
-        x, h = fused_gated_residual(x, self.attend(h, pos).to(x.dtype),
-                                    self.n2.weight, self.n2.bias,
-                                    gate=self.g1, eps=self.n2.eps)
-        return fused_gated_residual(x, self.mlp(h).to(x.dtype), after.weight,
-                                    after.bias, gate=self.g2, eps=after.eps)
 
 
 class GPT2(nn.Module):

@@ -8,13 +8,14 @@ import torch.nn.functional as F
 
 from ..ops.attn import fused_sdpa, fused_sdpa_qkv
 from ..ops.linear import FusedLinear
-from ..ops.ln import FusedLayerNorm, fused_gated_residual
+from ..ops.ln import FusedLayerNorm
 from ..ops.rope import AxialRotary
+from .block import TwoBranches
 
 
-class Block(nn.Module):
-    """rotary, layer_scale: as in the causal block (models/gpt2.py); rotary
-    turns by height and width."""
+class Block(TwoBranches):
+    """rotary : AxialRotary that turns q and k by height and width;
+    layer_scale : start value of the gates (models/block.py)."""
 
     def __init__(self, dim, heads, mlp_ratio=4.0, rotary=None,
                  layer_scale=None):
@@ -28,10 +29,7 @@ class Block(nn.Module):
         h = int(dim * mlp_ratio)
         self.fc1 = FusedLinear(dim, h)
         self.fc2 = FusedLinear(h, dim)
-        self.g1 = self.g2 = None
-        if layer_scale is not None:
-            self.g1 = nn.Parameter(torch.full((dim,), float(layer_scale)))
-            self.g2 = nn.Parameter(torch.full((dim,), float(layer_scale)))
+        self.add_gates(dim, layer_scale)
 
     def attend(self, h, pos=None):
         B, N, D = h.shape
@@ -44,29 +42,6 @@ class Block(nn.Module):
             y = fused_sdpa(q.transpose(1, 2), k.transpose(1, 2),
                            v.transpose(1, 2))
         return self.proj(y.transpose(1, 2).reshape(B, N, D))
-
-    def mlp(self, h):
-        return self.fc2(F.gelu(self.fc1(h)))
-
-    def forward(self, x, pos=None, h=None, after=None):
-        """x -> x behind this block; with h and ``after``: see ``joined``."""
-        if after is not None:
-            return self.joined(x, h, after, pos)
-        u = self.attend(self.n1(x), pos)
-        if self.g1 is None:
-            x = x + u
-            return x + self.mlp(self.n2(x))
-        x, h = fused_gated_residual(x, u.to(x.dtype), self.n2.weight,
-                                    self.n2.bias, gate=self.g1,
-                                    eps=self.n2.eps)
-        return x + self.g2 * self.mlp(h)
-
-    def joined(self, x, h, after, pos=None):
-        x, h = fused_gated_residual(x, self.attend(h, pos).to(x.dtype),
-                                    self.n2.weight, self.n2.bias,
-                                    gate=self.g1, eps=self.n2.eps)
-        return fused_gated_residual(x, self.mlp(h).to(x.dtype), after.weight,
-                                    after.bias, gate=self.g2, eps=after.eps)
 
 
 class ViT(nn.Module):
