@@ -63,12 +63,12 @@ def test_several_threads_on_streams_of_their_own():
     g = torch.Generator().manual_seed(0)
     rot = AxialRotary(64, (20, 12))
     pos = torch.stack([torch.arange(300), torch.arange(300) // 7]).to(DEV)
-    w = torch.randn(256, generator=g).bfloat16().to(DEV).requires_grad_()
+    weight = torch.randn(256, generator=g).bfloat16().to(DEV)
     inputs = [[torch.randn(2, 300, h, 64, generator=g).bfloat16().to(DEV)
                for h in (4, 2, 2, 4)] for _ in range(4)]
 
     def run(t):
-        q, k, v = (x.detach().requires_grad_() for x in t[:3])
+        q, k, v, w = (x.detach().requires_grad_() for x in (*t[:3], weight))
         a, b = rot(q, k, pos)
         o = fused_window_sdpa(a.transpose(1, 2), b.transpose(1, 2),
                               v.transpose(1, 2), 50, 3).transpose(1, 2)
