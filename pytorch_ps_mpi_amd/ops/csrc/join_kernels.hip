@@ -537,10 +537,10 @@ static void jn_pick(hipStream_t s, int grid, const JoinArgs& a) {
 }
 
 // Blocks of a group.  Backward 2048 waves: what the registers of most forms let
-// be on the chip at once; more would only write more parts.  Rows of at most 512
-// without Post leave room for 3072 to 5120, which 4096 waves use at 256 elements
-// (196608 rows: 294 us with 2048, 184 with 4096) and not at 512 (98304 rows: 117
-// and 125; with Post 118 and 125).  Forward 4096 waves: each
+// be on the chip at once (two a SIMD); more would only write more parts.  Rows of
+// at most 512 without Post leave room for three to five a SIMD, which 4096 waves
+// use at 256 elements (196608 rows: 294 us with 2048, 184 with 4096) and not at
+// 512 (98304 rows: 117 and 125; with Post 118 and 125).  Forward 4096 waves: each
 // reads the weights once (49152 rows of 768: 62 us with 8192, 58 with 4096).
 // Rows of 256 lanes with Post wait at more barriers and want 8192 (8192 rows of
 // 4096: 59 us with 4096, 55 with 8192; 16384 of 1536: 54 and 48), without Post
