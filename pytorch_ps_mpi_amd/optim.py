@@ -230,12 +230,12 @@ class PS(torch.optim.Optimizer):
         counts = {}
         for b in self.flat.buckets:
             c = {old.get(i, 0) for i, (s, e) in enumerate(zip(starts, ends))
-                 if s < b.end and b.start < e}
-            if len(c) != 1:
+                 if max(s, b.start) < min(e, b.end)}
+            if len(c) > 1:
                 raise ValueError(
                     f"elements {b.start} to {b.end} are one bucket here, in "
                     f"the checkpoint they had {sorted(c)} updates")
-            if c != {0}:
+            if c and c != {0}:  # none: a bucket without elements
                 counts[b.idx] = c.pop()
         return counts
 

@@ -81,3 +81,33 @@ def test_refused_checkpoint_leaves_the_seed():
         assert o2.seed == 9 and torch.equal(_flat(m), before)
     o2.load_state_dict(sd)
     assert o2.seed == 5
+
+
+@pytest.mark.parametrize("mb", [0, 0.0001, 50])
+def test_buckets_without_elements(mb):
+    """A parameter of no elements may be all of a bucket; no count is asked
+    of it."""
+    def made(mb):
+        torch.manual_seed(0)
+        named = [("none", torch.nn.Parameter(torch.zeros(0))),
+                 ("a", torch.nn.Parameter(torch.randn(300))),
+                 ("empty", torch.nn.Parameter(torch.zeros(0, 3))),
+                 ("b", torch.nn.Parameter(torch.randn(20)))]
+        return AdamW(named, lr=1e-2, bucket_mb=mb)
+
+    def train(o, steps):
+        for _ in range(steps):
+            o.zero_grad()
+            o.flat.flat_grad.copy_(o.flat.flat_param)
+            o.step()
+
+    o1 = made(0)
+    train(o1, 3)
+    o2 = made(mb)
+    o2.load_state_dict(o1.state_dict())
+    train(o2, 1)
+    o3 = made(50)
+    o3.load_state_dict(o2.state_dict())
+    train(o1, 3)
+    train(o3, 2)
+    assert torch.equal(o1.flat.master, o3.flat.master)
